@@ -51,7 +51,9 @@ typedef enum pd_dtype { PD_FLOAT16 = 0, PD_FLOAT32 = 1 } pd_dtype;
 /* Error-word bits a kernel can raise (read with pd_plan_read_errors). */
 #define PD_DEVERR_TIMEOUT 1u      /* a bounded wait on a shared-memory barrier ran out */
 #define PD_DEVERR_BAD_PAGE 2u     /* a live page id outside [0, physical_pages): tokens skipped */
-#define PD_DEVERR_LENGTH 8u       /* a dynamic launch's length exceeded the plan's max_lengths: clamped */
+#define PD_DEVERR_LENGTH 8u       /* a dynamic launch's length exceeded the plan's max_lengths: clamped;
+                                     an append's token lies outside its page table row: skipped */
+#define PD_DEVERR_POSITION 16u    /* a position outside the rotation table: the token is skipped */
 
 /* Replaces oracle.Layout (src/paged_decode/oracle.py:11-27). */
 typedef struct pd_layout {
@@ -322,6 +324,126 @@ pd_status pd_exchange_free(int32_t device, void *buffer);
 pd_status pd_decode_exchange(pd_plan *plan, const void *q, const void *k, const void *v, pd_dtype dtype,
                              void *const *buffers, int32_t rank, int32_t world, float *out, float *stats,
                              void *stream);
+
+/* ------------------------------------------------------------------------
+ * Heads on their way to the decode: RMS norm of each query and key head and
+ * the position rotation in one pass, alone (pd_rotate_heads) or while a step's
+ * keys and values are appended to the paged cache (pd_cache_append).  No
+ * reference counterpart (the reference starts from a filled cache).
+ *
+ * For a head row x with weight w:  y = x / sqrt(mean(x^2) + eps) * w  (skipped
+ * where w is NULL); then pairs (a, b) of its first rotary_dim elements become
+ * (a cos - b sin, b cos + a sin) with cos | sin = table[position], the rest
+ * passes.  FP32 inside, one rounding at the store.
+ */
+typedef struct pd_rotation {
+    int32_t head_dim;            /* 64 or 128 */
+    int32_t rotary_dim;          /* a multiple of 16 up to head_dim; unused without a table */
+    int32_t interleaved;         /* pairs: 0 (i, i + rotary_dim / 2), 1 (2i, 2i + 1) */
+    float eps;
+    int64_t max_positions;       /* rows of the table */
+    const float *table;          /* device, [max_positions][rotary_dim]: cos, then sin; NULL: no rotation */
+    const float *q_weight;       /* device, [head_dim]; NULL: queries are not normed */
+    const float *k_weight;       /* device, [head_dim]; NULL: keys are not normed */
+} pd_rotation;
+
+/* Rows [tokens][heads][head_dim] with any token and head stride (in elements,
+ * the last dim contiguous), e.g. a part of a packed projection. */
+typedef struct pd_heads {
+    const void *data;
+    int64_t token_stride, head_stride;
+    void *out;                   /* may be data itself, with the same strides */
+    int64_t out_token_stride, out_head_stride;
+    int32_t heads;               /* 0: no such rows */
+} pd_heads;
+
+/* q.out and k.out get the normed and rotated heads of token i at
+ * positions[i] (device int32 [tokens]).  A position outside the table leaves
+ * zero rows and flags PD_DEVERR_POSITION in *error (device word, caller-owned
+ * and zeroed).  q or k may be NULL.  Asynchronous, allocation-free, one launch. */
+pd_status pd_rotate_heads(const pd_rotation *rotation, const pd_heads *q, const pd_heads *k, int64_t tokens,
+                          const int32_t *positions, pd_dtype dtype, uint32_t *error, int32_t device,
+                          void *stream);
+
+/* Append new tokens to the paged caches [physical_pages, page_size, kv_heads,
+ * head_dim].  lengths (device int32 [batch]) already count the new tokens and
+ * table (device int32 [batch, table_width]) already names their pages, so both
+ * are what pd_decode_dynamic reads next.  With indptr (device int32 [batch +
+ * 1], indptr[0] = 0) tokens indptr[b] .. indptr[b + 1] - 1 are the last ones of
+ * sequence b, tokens from indptr[batch] on are padding; without it token b is
+ * the last one of sequence b, and a sequence of length 0 is not in use.  Keys
+ * are normed and rotated (rotation may be NULL: copied) at their position in
+ * the sequence, values are copied bit for bit; q (may be NULL) is normed and
+ * rotated into q.out.  Padding and skipped tokens write no cache row and
+ * leave zero query rows; a token outside its table row or the rotation table,
+ * or on a page outside the cache, is skipped and flags PD_DEVERR_LENGTH,
+ * PD_DEVERR_POSITION or PD_DEVERR_BAD_PAGE in *error.  k.out and v.out are not
+ * used.  Two tokens must not share a slot.  Asynchronous, allocation-free,
+ * one launch. */
+pd_status pd_cache_append(const pd_layout *layout, const pd_rotation *rotation, const pd_heads *q,
+                          const pd_heads *k, const pd_heads *v, int64_t tokens, void *k_cache, void *v_cache,
+                          pd_dtype dtype, const int32_t *table, int64_t table_width, const int32_t *lengths,
+                          const int32_t *indptr, uint32_t *error, int32_t device, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Shared-prefix decode: sequences whose page tables start with the same pages
+ * form a group, and the attention over those pages is computed once for the
+ * whole group (all members' query heads of a KV head as one matrix).  Each
+ * sequence's other pages are decoded as by pd_decode, and the two parts are
+ * merged by their softmax statistics.  Same inputs and meaning as pd_decode;
+ * out has the inputs' type (FP32 sums, rounded once).  No reference
+ * counterpart.
+ */
+typedef struct pd_prefix_plan pd_prefix_plan;
+
+typedef struct pd_prefix_info {
+    int32_t groups;              /* prefix groups */
+    int32_t members;             /* sequences in a group */
+    int32_t tile_rows;           /* query rows of one prefix tile */
+    int32_t items;               /* CTAs of the prefix kernel */
+    int32_t suffix_launch;       /* 1: the decode kernel runs (some sequence goes on behind its prefix) */
+    int32_t dynamic;
+    int64_t shared_pages;        /* page reads saved: sum over groups of (members - 1) * pages */
+    int64_t device_bytes;
+} pd_prefix_info;
+
+/* Build a plan from host metadata (see pd_plan_create; copied).  Groups: group
+ * g has members[indptr[g]] .. members[indptr[g + 1] - 1] (sequences, each in
+ * at most one group) sharing their first pages[g] pages, all of them whole
+ * (lengths >= pages * page_size) and equal in the table.  group_count < 0
+ * finds the groups in the table: leading pages that are worth sharing.
+ * max_lengths (NULL: a static plan) as in pd_plan_create_dynamic.  device < 0
+ * builds a host-only plan. */
+pd_status pd_prefix_plan_create(const pd_layout *layout, const int32_t *table, int64_t table_width,
+                                const int32_t *lengths, const int32_t *max_lengths, int32_t group_count,
+                                const int32_t *indptr, const int32_t *members, const int32_t *pages,
+                                pd_dtype dtype, int32_t device, pd_prefix_plan **out_plan);
+void pd_prefix_plan_destroy(pd_prefix_plan *plan);
+pd_status pd_prefix_plan_get_info(const pd_prefix_plan *plan, pd_prefix_info *info);
+
+/* The plan's groups: group[b] the group of sequence b or -1 (int32 [batch]),
+ * pages[g] its shared pages (int32 [groups]).  Either may be NULL. */
+pd_status pd_prefix_plan_copy_groups(const pd_prefix_plan *plan, int32_t *group, int32_t *pages);
+
+/* As pd_plan_device_bytes / pd_plan_bind. */
+size_t pd_prefix_plan_device_bytes(const pd_prefix_plan *plan);
+pd_status pd_prefix_plan_bind(pd_prefix_plan *plan, void *device_buffer, size_t bytes, void *stream);
+
+/* One decode step.  out [batch, query_heads, head_dim] in dtype, 16-byte
+ * aligned.  Asynchronous, allocation-free, may be captured in a CUDA graph;
+ * launches of one plan must stay in one stream order. */
+pd_status pd_prefix_decode(pd_prefix_plan *plan, const void *q, const void *k, const void *v, pd_dtype dtype,
+                           void *out, void *stream);
+
+/* One step of a dynamic plan with live metadata in device memory, as in
+ * pd_decode_dynamic.  The shared pages are the plan's; a sequence whose live
+ * length ends inside its prefix attends to its live tokens only. */
+pd_status pd_prefix_decode_dynamic(pd_prefix_plan *plan, const void *q, const void *k, const void *v,
+                                   pd_dtype dtype, const int32_t *table, const int32_t *lengths, void *out,
+                                   void *stream);
+
+/* Copy the plan's device error word to *error_word and clear it (synchronises `stream`). */
+pd_status pd_prefix_plan_read_errors(pd_prefix_plan *plan, uint32_t *error_word, void *stream);
 
 /* Diagnostics, no reference counterpart: runs the decode kernel's two kinds
  * of bounded wait against events that never happen -- an mbarrier phase that

@@ -349,7 +349,7 @@ pd_status max_active_pair_clusters(const pd_plan &p, int device, int *clusters) 
 pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t table_width,
                       const int32_t *lengths, const int32_t *max_lengths, int32_t split_tokens,
                       int32_t merge_mode, pd_dtype dtype, int32_t device, int32_t num_ctas,
-                      pd_plan **out_plan) {
+                      pd_plan **out_plan, const int32_t *first_pages = nullptr) {
     if (!out_plan) return fail(PD_ERR_VALUE, "out_plan must not be NULL");
     *out_plan = nullptr;
     int sm_count = 148;
@@ -361,7 +361,7 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t tab
     pd_plan *p = new (std::nothrow) pd_plan();
     if (!p) return fail(PD_ERR_VALUE, "out of host memory");
     pd_status s = build_plan(layout, table, table_width, lengths, max_lengths, split_tokens, merge_mode,
-                             dtype, num_ctas, sm_count, *p);
+                             dtype, num_ctas, sm_count, *p, true, first_pages);
     if (s == PD_OK && p->cluster == 2 && device >= 0) {
         // A pair plan only where all its clusters of two CTAs fit on the device
         // at once (shared memory, GPC boundaries); otherwise one CTA per SM.
@@ -370,7 +370,7 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t tab
         if (s == PD_OK && 2 * int64_t(clusters) < p->num_ctas) {
             *p = pd_plan();
             s = build_plan(layout, table, table_width, lengths, max_lengths, split_tokens, merge_mode, dtype,
-                           num_ctas, sm_count, *p, false);
+                           num_ctas, sm_count, *p, false, first_pages);
         }
     }
     if (s != PD_OK) {
@@ -382,6 +382,13 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t tab
     return PD_OK;
 }
 }  // namespace
+
+pd_status pd::create_suffix_plan(const pd_layout *layout, const int32_t *table, int64_t table_width,
+                                 const int32_t *lengths, const int32_t *max_lengths, const int32_t *first_pages,
+                                 pd_dtype dtype, int32_t device, pd_plan **out_plan) {
+    return create_impl(layout, table, table_width, lengths, max_lengths, 256, 0, dtype, device, 0, out_plan,
+                       first_pages);
+}
 
 PD_API pd_status pd_plan_create(const pd_layout *layout, const int32_t *table, int64_t table_width,
                                 const int32_t *lengths, int32_t split_tokens, int32_t merge_mode,

@@ -45,7 +45,7 @@ const std::string &last_error() { return g_last_error; }
 pd_status build_plan(const pd_layout *layout, const int32_t *table, int64_t width,
                      const int32_t *lengths, const int32_t *max_lengths, int32_t split_tokens,
                      int32_t merge_mode, pd_dtype dtype, int32_t num_ctas, int32_t sm_count,
-                     pd_plan &p, bool allow_pair) {
+                     pd_plan &p, bool allow_pair, const int32_t *first_pages) {
     if (!layout) return fail(PD_ERR_VALUE, "layout must not be NULL");
     const pd_layout L = *layout;
     // Layout.__post_init__ (oracle.py:24-27)
@@ -91,6 +91,12 @@ pd_status build_plan(const pd_layout *layout, const int32_t *table, int64_t widt
         for (int b = 0; b < L.batch; ++b)
             if (max_lengths[b] < lengths[b] || max_lengths[b] > capacity)
                 return fail(PD_ERR_VALUE, "max_lengths must lie between lengths and the page table capacity");
+    // A suffix plan's work starts at page first_pages[b] of each sequence.
+    if (first_pages)
+        for (int b = 0; b < L.batch; ++b)
+            if (first_pages[b] < 0 || first_pages[b] > width)
+                return fail(PD_ERR_VALUE, "first_pages must lie within the page table");
+    const auto first_page = [&](int b) { return first_pages ? int64_t(first_pages[b]) : int64_t(0); };
     const int32_t *span = max_lengths ? max_lengths : lengths;
     int32_t max_context = 0, max_span = 0;
     for (int b = 0; b < L.batch; ++b) {
@@ -166,7 +172,7 @@ pd_status build_plan(const pd_layout *layout, const int32_t *table, int64_t widt
                 g[4] = span[b];                        // tokens the group's work covers
                 g[5] = -1;
                 g[6] = 0;
-                gpages[gi] = (int64_t(span[b]) + T - 1) / T;
+                gpages[gi] = std::max<int64_t>(0, (int64_t(span[b]) + T - 1) / T - first_page(b));
                 total += gpages[gi];
             }
     if (total > INT32_MAX) return fail(PD_ERR_VALUE, "too many page tiles per decode step");
@@ -241,6 +247,14 @@ pd_status build_plan(const pd_layout *layout, const int32_t *table, int64_t widt
         }
         cursor = end;
     }
+    // Segments name the table's columns: a suffix plan's work starts at first_page(b).
+    if (first_pages)
+        for (auto &v : per)
+            for (size_t k = 0; k < v.size(); k += 4) {
+                const int32_t first = int32_t(first_page(p.groups[size_t(v[k]) * 8]));
+                v[k + 1] += first;
+                v[k + 2] += first;
+            }
     // Partial slots.  A segment's consumer warps may run as several
     // sub-pipelines (alternate page tiles).  Kernel shapes that fold their
     // states inside the CTA (fold_sub_pipelines) write one partial slot per

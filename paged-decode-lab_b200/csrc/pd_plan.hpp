@@ -85,9 +85,16 @@ namespace pd {
 // sequence b up to max_lengths[b] tokens, and launches may pass live lengths
 // <= max_lengths and a page table updated on the device.
 // `allow_pair` = false never builds a pair plan (clusters of two CTAs).
+// `first_pages` (nullable) makes a suffix plan: sequence b's work starts at its
+// logical page first_pages[b] (tokens before it take no part).
 pd_status build_plan(const pd_layout *layout, const int32_t *table, int64_t width,
                      const int32_t *lengths, const int32_t *max_lengths, int32_t split_tokens,
                      int32_t merge_mode, pd_dtype dtype, int32_t num_ctas, int32_t sm_count,
-                     pd_plan &plan, bool allow_pair = true);
+                     pd_plan &plan, bool allow_pair = true, const int32_t *first_pages = nullptr);
+
+// A decode plan of the sequences' pages from first_pages[b] on.
+pd_status create_suffix_plan(const pd_layout *layout, const int32_t *table, int64_t width, const int32_t *lengths,
+                             const int32_t *max_lengths, const int32_t *first_pages, pd_dtype dtype, int32_t device,
+                             pd_plan **out_plan);
 
 }  // namespace pd

@@ -1,0 +1,68 @@
+// pd_prefix.hpp — plans of shared-prefix decode attention (host side).
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <vector>
+
+#include "paged_decode.h"
+#include "pd_plan.hpp"
+
+namespace pd {
+
+// Sections of the plan's device buffer (256-byte aligned).
+struct PrefixImage {
+    size_t off_error = 0, off_items = 0, off_seqs = 0, off_members = 0, off_pages = 0, off_lengths = 0;
+    size_t off_suffix = 0;                        // the suffix plan's own buffer
+    size_t off_rows = 0, off_stats = 0;           // the suffix decode's FP32 rows and (m, l)
+    size_t off_part_o = 0, off_part_ml = 0;       // the prefix pieces' partials
+    size_t metadata = 0, bytes = 0;
+};
+
+struct PrefixGroup {
+    std::vector<int32_t> members;   // sequences, ascending
+    int32_t pages = 0;              // shared leading pages
+};
+
+}  // namespace pd
+
+struct pd_prefix_plan {
+    pd_layout layout{};
+    pd_dtype dtype = PD_FLOAT16;
+    int32_t device = -1;
+    int64_t width = 0;
+    int32_t group = 0;              // G = Hq / Hkv
+    int32_t tile_rows = 0;          // query rows of one prefix tile
+    int32_t slots = 0;              // partial slots (tile pieces)
+    bool dynamic = false;
+    bool suffix_empty = false;      // no sequence has pages past its prefix: nothing for the decode kernel
+    std::vector<pd::PrefixGroup> groups;
+    std::vector<int32_t> items;     // 8 per work item, see PrefixArgs::items
+    std::vector<int32_t> seqs;      // 4 per sequence, see PrefixArgs::seqs
+    pd_plan *suffix = nullptr;
+    pd::PrefixImage image;
+    std::vector<uint8_t> host_image;
+    uint8_t *dev = nullptr;
+    const void *k = nullptr, *v = nullptr;   // the caches the tensor maps describe
+    alignas(64) CUtensorMap map_k, map_v;
+
+    ~pd_prefix_plan() { delete suffix; }
+};
+
+namespace pd {
+
+// Groups of sequences whose leading pages are the same.  A candidate is all
+// sequences that start with some pages; disjoint candidates are chosen so that
+// the page reads saved, less `overhead_pages` per group, are the most.
+void find_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,
+                        int64_t overhead_pages, std::vector<PrefixGroup> &groups);
+
+// Check the groups against the table and lengths.
+pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,
+                              const std::vector<PrefixGroup> &groups);
+
+// Lay the groups' work out over the device and build the device image; the
+// suffix plan is set.
+pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count);
+
+}  // namespace pd

@@ -13,7 +13,7 @@ LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 
 PD_OK, PD_ERR_VALUE, PD_ERR_TYPE, PD_ERR_CUDA, PD_ERR_DEVICE, PD_ERR_UNBOUND = range(6)
 PD_FLOAT16, PD_FLOAT32 = 0, 1
-PD_DEVERR_TIMEOUT, PD_DEVERR_BAD_PAGE = 1, 2
+PD_DEVERR_TIMEOUT, PD_DEVERR_BAD_PAGE, PD_DEVERR_LENGTH, PD_DEVERR_POSITION = 1, 2, 8, 16
 PD_BARRIER_PLAIN, PD_BARRIER_COOPERATIVE, PD_BARRIER_LEAVE_AT_ONCE = 0, 1, 2
 PD_ENGINE_WARP, PD_ENGINE_TCGEN05 = 0, 1
 
@@ -38,6 +38,24 @@ class PlanInfo(ctypes.Structure):
                 ("dynamic", ctypes.c_int32), ("max_span", ctypes.c_int32),
                 ("workspace_bytes", ctypes.c_int64), ("device_bytes", ctypes.c_int64),
                 ("engine", ctypes.c_int32), ("cluster_ctas", ctypes.c_int32)]
+
+
+class PrefixInfo(ctypes.Structure):
+    _fields_ = [("groups", ctypes.c_int32), ("members", ctypes.c_int32), ("tile_rows", ctypes.c_int32),
+                ("items", ctypes.c_int32), ("suffix_launch", ctypes.c_int32), ("dynamic", ctypes.c_int32),
+                ("shared_pages", ctypes.c_int64), ("device_bytes", ctypes.c_int64)]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("max_positions", ctypes.c_int64), ("table", ctypes.c_void_p),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p)]
+
+
+class Heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_token_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("heads", ctypes.c_int32)]
 
 
 SIGNATURES = {
@@ -73,6 +91,19 @@ SIGNATURES = {
     "pd_status_string": (ctypes.c_char_p, [_c_int32]),
     "pd_last_error": (ctypes.c_char_p, []),
     "pd_abi_version": (_c_int32, []),
+    "pd_rotate_heads": (_c_int32, [_vp, _vp, _vp, _c_int64, _vp, _c_int32, _vp, _c_int32, _vp]),
+    "pd_cache_append": (_c_int32, [_vp, _vp, _vp, _vp, _vp, _c_int64, _vp, _vp, _c_int32, _vp, _c_int64, _vp,
+                                   _vp, _vp, _c_int32, _vp]),
+    "pd_prefix_plan_create": (_c_int32, [ctypes.POINTER(Layout), _vp, _c_int64, _vp, _vp, _c_int32, _vp, _vp, _vp,
+                                         _c_int32, _c_int32, ctypes.POINTER(_vp)]),
+    "pd_prefix_plan_destroy": (None, [_vp]),
+    "pd_prefix_plan_get_info": (_c_int32, [_vp, ctypes.POINTER(PrefixInfo)]),
+    "pd_prefix_plan_copy_groups": (_c_int32, [_vp, _vp, _vp]),
+    "pd_prefix_plan_device_bytes": (_c_size, [_vp]),
+    "pd_prefix_plan_bind": (_c_int32, [_vp, _vp, _c_size, _vp]),
+    "pd_prefix_decode": (_c_int32, [_vp, _vp, _vp, _vp, _c_int32, _vp, _vp]),
+    "pd_prefix_decode_dynamic": (_c_int32, [_vp, _vp, _vp, _vp, _c_int32, _vp, _vp, _vp, _vp]),
+    "pd_prefix_plan_read_errors": (_c_int32, [_vp, ctypes.POINTER(ctypes.c_uint32), _vp]),
     "pd_selftest_wait_timeouts": (_c_int32, [_c_int32, ctypes.c_uint32, _vp]),
     "pd_selftest_barrier_leave": (_c_int32, [_c_int32, ctypes.c_uint32, _vp]),
 }
