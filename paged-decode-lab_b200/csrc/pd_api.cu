@@ -383,6 +383,12 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t tab
 }
 }  // namespace
 
+pd_status pd::encode_prefix_maps(const pd_plan &plan, const void *k, const void *v, CUtensorMap *map_k,
+                                 CUtensorMap *map_v) {
+    const pd_status s = encode_cache_map(plan, k, plan.dtype, 1, map_k, true);
+    return s == PD_OK ? encode_cache_map(plan, v, plan.dtype, 1, map_v) : s;
+}
+
 pd_status pd::create_suffix_plan(const pd_layout *layout, const int32_t *table, int64_t table_width,
                                  const int32_t *lengths, const int32_t *max_lengths, const int32_t *first_pages,
                                  pd_dtype dtype, int32_t device, pd_plan **out_plan) {

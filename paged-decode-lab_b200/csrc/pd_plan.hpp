@@ -97,4 +97,9 @@ pd_status create_suffix_plan(const pd_layout *layout, const int32_t *table, int6
                              const int32_t *max_lengths, const int32_t *first_pages, pd_dtype dtype, int32_t device,
                              pd_plan **out_plan);
 
+// One-head page views of the caches as the tcgen05 kernels read them: K in
+// 8-token groups, V token by token.
+pd_status encode_prefix_maps(const pd_plan &plan, const void *k, const void *v, CUtensorMap *map_k,
+                             CUtensorMap *map_v);
+
 }  // namespace pd

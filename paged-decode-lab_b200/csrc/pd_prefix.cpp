@@ -115,43 +115,122 @@ pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int
     return PD_OK;
 }
 
+namespace {
+
+// FP32 (CUDA cores): tiles of 16 rows, pieces of whole 32-token steps, about
+// four CTAs per SM in all.
+struct SimtShape {
+    static constexpr int64_t rows = 16, step_tokens = 32, ctas_per_sm = 4;
+};
+
+// FP16 (tcgen05): tiles of 128 rows, 128-token steps, one CTA per SM with two
+// streams (see pd_prefix_mma.cuh).
+struct MmaShape {
+    static constexpr int64_t rows = 128, step_tokens = 128;
+    // start and end of a CTA (launch, first loads, the partials' store), in steps
+    static constexpr int64_t overhead_steps = 3;
+};
+
+}  // namespace
+
 pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count) {
     const pd_layout &L = p.layout;
     const int D = L.head_dim;
+    const bool mma = p.dtype == PD_FLOAT16;
     p.group = L.query_heads / L.kv_heads;
-    p.tile_rows = 16;
-    const int64_t step_pages = std::max(1, 32 / L.page_size);
-    int64_t tiles = 0;
-    for (const PrefixGroup &g : p.groups)
-        tiles += int64_t(L.kv_heads) * ((int64_t(g.members.size()) * p.group + p.tile_rows - 1) / p.tile_rows);
-    p.seqs.assign(size_t(L.batch) * 4, 0);
-    for (int b = 0; b < L.batch; ++b) p.seqs[size_t(b) * 4] = -1;
-    p.items.clear();
-    std::vector<int32_t> members, pages;
-    int64_t slots = 0;
-    for (const PrefixGroup &g : p.groups) {
-        const int64_t rows = int64_t(g.members.size()) * p.group;
-        const int64_t ntiles = (rows + p.tile_rows - 1) / p.tile_rows;
-        const int64_t steps = (g.pages + step_pages - 1) / step_pages;
-        const int64_t pieces = std::min(steps, std::max<int64_t>(1, (4 * int64_t(sm_count) + tiles - 1) / tiles));
-        for (size_t j = 0; j < g.members.size(); ++j) {
-            int32_t *s = &p.seqs[size_t(g.members[j]) * 4];
-            s[0] = int32_t(j);
-            s[1] = int32_t(slots);
-            s[2] = int32_t(ntiles);
-            s[3] = int32_t(pieces);
+    p.tile_rows = int32_t(mma ? MmaShape::rows : SimtShape::rows);
+    p.item_words = mma ? 16 : 8;
+    const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtShape::step_tokens) / L.page_size;
+    const auto tiles_of = [&](const PrefixGroup &g) {
+        return (int64_t(g.members.size()) * p.group + p.tile_rows - 1) / p.tile_rows;
+    };
+    const auto steps_of = [&](const PrefixGroup &g) { return (g.pages + step_pages - 1) / step_pages; };
+    // Steps per work item: FP16 takes what finishes first when the CTAs run in
+    // waves of one per SM and each costs its steps and the fixed overhead.
+    int64_t item_steps = 1;
+    if (mma) {
+        int64_t most = 1, best = INT64_MAX;
+        for (const PrefixGroup &g : p.groups) most = std::max<int64_t>(most, steps_of(g));
+        const auto items = [&](int64_t steps) {
+            int64_t n = 0;
+            for (const PrefixGroup &g : p.groups) {
+                const int64_t t = tiles_of(g), s = steps_of(g);
+                n += L.kv_heads * (t / 2 * ((s + steps - 1) / steps) + t % 2 * ((s + 2 * steps - 1) / (2 * steps)));
+            }
+            return n;
+        };
+        for (int64_t steps = 1; steps <= most; ++steps) {
+            const int64_t waves = (items(steps) + sm_count - 1) / sm_count;
+            const int64_t cost = waves * (MmaShape::overhead_steps + steps);
+            if (cost < best) best = cost, item_steps = steps;
         }
-        if (slots + int64_t(L.kv_heads) * ntiles * pieces > INT32_MAX / 256)
-            return fail(PD_ERR_VALUE, "too many prefix tiles");
-        for (int h = 0; h < L.kv_heads; ++h)
-            for (int64_t t = 0; t < ntiles; ++t)
-                for (int64_t c = 0; c < pieces; ++c, ++slots) {
-                    const int64_t first = c * steps / pieces * step_pages;
-                    const int64_t end = std::min<int64_t>(g.pages, (c + 1) * steps / pieces * step_pages);
-                    p.items.insert(p.items.end(),
-                                   {int32_t(members.size()), int32_t(g.members.size()), h, int32_t(t),
-                                    int32_t(pages.size()), int32_t(first), int32_t(end), int32_t(slots)});
+    } else {
+        int64_t work = 0;
+        for (const PrefixGroup &g : p.groups) work += L.kv_heads * tiles_of(g) * steps_of(g);
+        item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, SimtShape::ctas_per_sm * sm_count));
+    }
+    p.seqs.assign(size_t(L.batch) * 8, 0);
+    for (int b = 0; b < L.batch; ++b) p.seqs[size_t(b) * 8] = -1;
+    p.items.clear();
+    p.tiles.clear();
+    std::vector<int32_t> members, pages;
+    int64_t slots = 0, count = 0;
+    for (const PrefixGroup &g : p.groups) {
+        const int64_t ntiles = tiles_of(g), steps = steps_of(g);
+        count += L.kv_heads * ntiles * steps;
+        if (count > INT32_MAX / 1024) return fail(PD_ERR_VALUE, "too many prefix tiles");
+        for (size_t j = 0; j < g.members.size(); ++j) {
+            int32_t *s = &p.seqs[size_t(g.members[j]) * 8];
+            s[0] = int32_t(j);
+            s[1] = int32_t(p.tiles.size() / 2);
+            s[2] = int32_t(ntiles);
+            s[3] = int32_t(pages.size());
+            s[4] = g.pages;
+        }
+        const int32_t m0 = int32_t(members.size()), n = int32_t(g.members.size()), pg = int32_t(pages.size());
+        // piece c of `pieces`: whole steps, as even as they come
+        const auto bound = [&](int64_t c, int64_t pieces) {
+            return int32_t(std::min<int64_t>(g.pages, c * steps / pieces * step_pages));
+        };
+        for (int h = 0; h < L.kv_heads; ++h) {
+            for (int64_t t = 0; t < ntiles; ++t) {
+                const bool paired = mma && (t ^ 1) < ntiles;
+                const bool split = mma && !paired && steps > 1;
+                int64_t pieces = (steps + item_steps - 1) / item_steps;
+                if (split) pieces = (steps + 2 * item_steps - 1) / (2 * item_steps) * 2;
+                pieces = std::min(pieces, steps);
+                p.tiles.insert(p.tiles.end(), {int32_t(slots), int32_t(pieces)});
+                const int32_t slot = int32_t(slots), tile = int32_t(t);
+                slots += pieces;
+                if (!mma) {
+                    for (int64_t c = 0; c < pieces; ++c)
+                        p.items.insert(p.items.end(), {m0, n, h, tile, pg, bound(c, pieces), bound(c + 1, pieces),
+                                                       int32_t(slot + c)});
+                } else if (!paired) {
+                    // two neighbouring pieces of one tile, the longer one first
+                    for (int64_t c = 0; c < pieces; c += 2) {
+                        int32_t x[4] = {bound(c, pieces), bound(c + 1, pieces), 0, 0};
+                        int32_t sx = int32_t(slot + c), sy = sx;
+                        if (c + 1 < pieces) {
+                            x[2] = x[1], x[3] = bound(c + 2, pieces), sy = sx + 1;
+                            if (x[3] - x[2] > x[1] - x[0]) {
+                                std::swap(x[0], x[2]);
+                                std::swap(x[1], x[3]);
+                                std::swap(sx, sy);
+                            }
+                        }
+                        p.items.insert(p.items.end(), {m0, n, h, 0, pg, 0, 0, 0, tile, x[0], x[1], sx, tile, x[2], x[3], sy});
+                    }
+                } else if (t % 2) {
+                    // both tiles of a pair have the same pieces; this one's slots follow the other's
+                    for (int64_t c = 0; c < pieces; ++c)
+                        p.items.insert(p.items.end(),
+                                       {m0, n, h, 1, pg, 0, 0, 0, tile - 1, bound(c, pieces), bound(c + 1, pieces),
+                                        int32_t(slot - pieces + c), tile, bound(c, pieces), bound(c + 1, pieces),
+                                        int32_t(slot + c)});
                 }
+            }
+        }
         members.insert(members.end(), g.members.begin(), g.members.end());
         const int32_t *row = table + int64_t(g.members[0]) * p.width;
         pages.insert(pages.end(), row, row + g.pages);
@@ -163,6 +242,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     im.off_error = off;    off = align256(off + 4);
     im.off_items = off;    off = align256(off + p.items.size() * 4);
     im.off_seqs = off;     off = align256(off + p.seqs.size() * 4);
+    im.off_tiles = off;    off = align256(off + p.tiles.size() * 4);
     im.off_members = off;  off = align256(off + members.size() * 4);
     im.off_pages = off;    off = align256(off + pages.size() * 4);
     im.off_lengths = off;  off = align256(off + size_t(L.batch) * 4);
@@ -179,6 +259,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     };
     put(im.off_items, p.items.data(), p.items.size() * 4);
     put(im.off_seqs, p.seqs.data(), p.seqs.size() * 4);
+    put(im.off_tiles, p.tiles.data(), p.tiles.size() * 4);
     put(im.off_members, members.data(), members.size() * 4);
     put(im.off_pages, pages.data(), pages.size() * 4);
     put(im.off_lengths, lengths, size_t(L.batch) * 4);

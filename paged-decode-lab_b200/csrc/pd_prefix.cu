@@ -15,6 +15,7 @@
 #include "pd_device.cuh"
 #include "pd_prefix.hpp"
 #include "pd_prefix_args.cuh"
+#include "pd_prefix_mma.cuh"
 
 #define PD_API extern "C" __attribute__((visibility("default")))
 
@@ -30,13 +31,6 @@ template <>
 __device__ __forceinline__ float4 load4<float>(const float *p) {
     return __ldcg(reinterpret_cast<const float4 *>(p));
 }
-template <>
-__device__ __forceinline__ float4 load4<__half>(const __half *p) {
-    const uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
-    const float2 a = unpack_half2(v.x), b = unpack_half2(v.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-
 // One CTA per work item: 16 query rows of one KV head against a piece of the
 // prefix, 32 tokens a step.  Eight threads per row: each scores every eighth
 // token, then adds up its eighth of the head's dims.
@@ -135,6 +129,38 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// (m, l) of one row over the first `limit` tokens of its prefix, o in `o`: for a
+// dynamic launch's sequence that ends inside its prefix, whose row in the
+// group's matrix covers the whole prefix.  One warp, a token at a time: such
+// lengths are rare, and most of them 0.
+template <typename Elt, int D>
+__device__ __noinline__ float2 prefix_row(const PrefixArgs &a, int64_t row, int kv_head, const int32_t *pages,
+                                          int limit, int lane, float (&o)[D / 32]) {
+    constexpr int N = D / 32;
+    float q[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        q[i] = float(static_cast<const Elt *>(a.q)[row * D + lane * N + i]) * a.scale_log2;
+        o[i] = 0.f;
+    }
+    for (int t = 0; t < limit; ++t) {
+        const int64_t at = ((int64_t(pages[t / a.page_size]) * a.page_size + t % a.page_size) * a.Hkv + kv_head) * D +
+                           lane * N;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s = fmaf(q[i], float(static_cast<const Elt *>(a.k)[at + i]), s);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(kFullMask, s, x);
+        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
+        const float shrink = exp2f(m - base), p = exp2f(s - base);
+        l = fmaf(l, shrink, p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(o[i], shrink, p * float(static_cast<const Elt *>(a.v)[at + i]));
+        m = top;
+    }
+    return make_float2(m, l);
+}
+
 // One warp per output row: the suffix's normalised row and the prefix pieces,
 // in piece order, each scaled to the common maximum.
 template <typename Elt, int D>
@@ -145,19 +171,30 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
     const int lane = threadIdx.x & 31;
     constexpr int N = D / 32;                                   // dims per lane
     const int b = int(out_row / a.Hq), head = int(out_row % a.Hq);
-    const int4 sq = a.seqs[b];
-    const int pieces = sq.x < 0 ? 0 : sq.w;
+    const int4 sq = a.seqs[2 * b];
     int64_t slot = 0;
-    int r = 0;
-    if (pieces) {
+    int r = 0, pieces = 0;
+    float2 own = make_float2(-INFINITY, 0.f);                   // a prefix part computed here
+    float oo[N];
+    if (sq.x >= 0) {
         const int row = sq.x * a.group + head % a.group;
-        slot = sq.y + (int64_t(head / a.group) * sq.z + row / a.tile_rows) * pieces;
+        const int2 tile = a.tiles[sq.y + int64_t(head / a.group) * sq.z + row / a.tile_rows];
+        slot = tile.x;
+        pieces = tile.y;
         r = row % a.tile_rows;
+        if constexpr (sizeof(Elt) == 2) {
+            const int limit = __ldcg(a.lengths + b);
+            if (limit < a.seqs[2 * b + 1].x * a.page_size) {
+                pieces = 0;
+                own = prefix_row<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, limit, lane, oo);
+            }
+        }
     }
     float2 suffix = make_float2(-INFINITY, 0.f);
     if (a.rows) suffix = reinterpret_cast<const float2 *>(a.stats)[out_row];
     // parts with no token have l = 0; a NaN denominator stays one
     float top = suffix.y != 0.f ? suffix.x : -INFINITY;
+    if (own.y != 0.f) top = fmaxf(top, own.x);
     for (int p = 0; p < pieces; ++p) {
         const float2 ml = a.part_ml[(slot + p) * a.tile_rows + r];
         if (ml.y != 0.f) top = fmaxf(top, ml.x);
@@ -170,6 +207,12 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
         const float *x = a.rows + out_row * D + lane * N;
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = den * x[i];
+    }
+    if (own.y != 0.f) {
+        const float w = exp2f(own.x - top);
+        den = fmaf(w, own.y, den);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fmaf(w, oo[i], o[i]);
     }
     for (int p = 0; p < pieces; ++p) {
         const int64_t at = (slot + p) * a.tile_rows + r;
@@ -187,11 +230,11 @@ __global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
     for (int i = 0; i < N; ++i) dst[i] = Elt(o[i] * inv);
 }
 
-template <typename Kernel>
-cudaError_t launch_dependent(Kernel kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
-                             const PrefixArgs &a) {
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, unsigned threads, size_t smem,
+                             cudaStream_t stream, const Args &...args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = dim3(unsigned(grid));
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -200,17 +243,39 @@ cudaError_t launch_dependent(Kernel kernel, unsigned grid, unsigned threads, siz
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <typename Elt, int D>
-cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, cudaStream_t stream) {
-    if (!p.items.empty()) {
-        const cudaError_t err = launch_dependent(prefix_simt_kernel<Elt, D>, unsigned(p.items.size() / 8), kSimtThreads,
-                                                 0, stream, a);
-        if (err != cudaSuccess) return err;
+using MmaKernel = void (*)(const CUtensorMap, const CUtensorMap, const PrefixArgs);
+struct MmaEntry {
+    MmaKernel kernel;
+    unsigned threads;
+    size_t smem;
+};
+template <int D, int T>
+MmaEntry mma_entry() {
+    return {prefix_mma_kernel<D, T>, PrefixShape<D, T>::THREADS, PrefixShape<D, T>::SMEM};
+}
+MmaEntry mma_entry_for(const pd_layout &L) {
+    if (L.head_dim == 64) return L.page_size == 16 ? mma_entry<64, 16>() : mma_entry<64, 32>();
+    return L.page_size == 16 ? mma_entry<128, 16>() : mma_entry<128, 32>();
+}
+
+template <int D>
+cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CUtensorMap &map_k,
+                          const CUtensorMap &map_v, cudaStream_t stream) {
+    cudaError_t err = cudaSuccess;
+    const int64_t items = int64_t(p.items.size()) / p.item_words;
+    if (items && p.dtype == PD_FLOAT16) {
+        const MmaEntry e = mma_entry_for(p.layout);
+        err = launch_dependent(e.kernel, items, e.threads, e.smem, stream, map_k, map_v, a);
+    } else if (items) {
+        err = launch_dependent(prefix_simt_kernel<float, D>, items, kSimtThreads, 0, stream, a);
     }
-    return launch_dependent(prefix_merge_kernel<Elt, D>, unsigned((int64_t(a.B) * a.Hq + 7) / 8), 256, 0, stream, a);
+    if (err != cudaSuccess) return err;
+    const int64_t grid = (int64_t(a.B) * a.Hq + 7) / 8;
+    return p.dtype == PD_FLOAT16 ? launch_dependent(prefix_merge_kernel<__half, D>, grid, 256, 0, stream, a)
+                                 : launch_dependent(prefix_merge_kernel<float, D>, grid, 256, 0, stream, a);
 }
 
 pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const void *v, pd_dtype dtype,
@@ -234,6 +299,7 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.v = v;
     a.items = reinterpret_cast<const int4 *>(p->dev + im.off_items);
     a.seqs = reinterpret_cast<const int4 *>(p->dev + im.off_seqs);
+    a.tiles = reinterpret_cast<const int2 *>(p->dev + im.off_tiles);
     a.members = reinterpret_cast<const int32_t *>(p->dev + im.off_members);
     a.pages = reinterpret_cast<const int32_t *>(p->dev + im.off_pages);
     a.lengths = lengths ? lengths : reinterpret_cast<const int32_t *>(p->dev + im.off_lengths);
@@ -250,7 +316,9 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.P = p->layout.physical_pages;
     a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(p->layout.head_dim)));
     pd_status s = PD_OK;
-    if (!p->suffix_empty) {
+    alignas(64) CUtensorMap map_k, map_v;
+    if (dtype == PD_FLOAT16 && !p->items.empty()) s = encode_prefix_maps(*p->suffix, k, v, &map_k, &map_v);
+    if (s == PD_OK && !p->suffix_empty) {
         float *rows = reinterpret_cast<float *>(p->dev + im.off_rows);
         float *stats = reinterpret_cast<float *>(p->dev + im.off_stats);
         s = table ? pd_decode_dynamic(p->suffix, q, k, v, dtype, table, lengths, rows, stats, stream)
@@ -260,10 +328,8 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     }
     if (s == PD_OK) {
         const auto st = static_cast<cudaStream_t>(stream);
-        if (dtype == PD_FLOAT16)
-            err = p->layout.head_dim == 64 ? launch_prefix<__half, 64>(*p, a, st) : launch_prefix<__half, 128>(*p, a, st);
-        else
-            err = p->layout.head_dim == 64 ? launch_prefix<float, 64>(*p, a, st) : launch_prefix<float, 128>(*p, a, st);
+        err = p->layout.head_dim == 64 ? launch_prefix<64>(*p, a, map_k, map_v, st)
+                                       : launch_prefix<128>(*p, a, map_k, map_v, st);
         if (err != cudaSuccess) s = fail(PD_ERR_CUDA, std::string("prefix launch: ") + cudaGetErrorString(err));
     }
     if (prev >= 0 && prev != p->device) cudaSetDevice(prev);
@@ -346,7 +412,7 @@ PD_API pd_status pd_prefix_plan_get_info(const pd_prefix_plan *p, pd_prefix_info
         info->shared_pages += int64_t(g.members.size() - 1) * g.pages;
     }
     info->tile_rows = p->tile_rows;
-    info->items = int32_t(p->items.size() / 8);
+    info->items = int32_t(p->items.size() / p->item_words);
     info->suffix_launch = p->suffix_empty ? 0 : 1;
     info->dynamic = p->dynamic ? 1 : 0;
     info->device_bytes = int64_t(p->image.bytes);
@@ -380,6 +446,11 @@ PD_API pd_status pd_prefix_plan_bind(pd_prefix_plan *p, void *buffer, size_t byt
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
     cudaError_t err = prev == p->device ? cudaSuccess : cudaSetDevice(p->device);
     const auto st = static_cast<cudaStream_t>(stream);
+    if (err == cudaSuccess && p->dtype == PD_FLOAT16) {
+        const MmaEntry e = mma_entry_for(p->layout);
+        err = cudaFuncSetAttribute(reinterpret_cast<const void *>(e.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   int(e.smem));
+    }
     if (err == cudaSuccess)
         err = cudaMemcpyAsync(dev, p->host_image.data(), p->host_image.size(), cudaMemcpyHostToDevice, st);
     if (err == cudaSuccess) err = cudaStreamSynchronize(st);

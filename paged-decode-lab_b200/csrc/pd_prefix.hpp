@@ -12,7 +12,7 @@ namespace pd {
 
 // Sections of the plan's device buffer (256-byte aligned).
 struct PrefixImage {
-    size_t off_error = 0, off_items = 0, off_seqs = 0, off_members = 0, off_pages = 0, off_lengths = 0;
+    size_t off_error = 0, off_items = 0, off_seqs = 0, off_tiles = 0, off_members = 0, off_pages = 0, off_lengths = 0;
     size_t off_suffix = 0;                        // the suffix plan's own buffer
     size_t off_rows = 0, off_stats = 0;           // the suffix decode's FP32 rows and (m, l)
     size_t off_part_o = 0, off_part_ml = 0;       // the prefix pieces' partials
@@ -37,14 +37,14 @@ struct pd_prefix_plan {
     bool dynamic = false;
     bool suffix_empty = false;      // no sequence has pages past its prefix: nothing for the decode kernel
     std::vector<pd::PrefixGroup> groups;
-    std::vector<int32_t> items;     // 8 per work item, see PrefixArgs::items
-    std::vector<int32_t> seqs;      // 4 per sequence, see PrefixArgs::seqs
+    int32_t item_words = 0;
+    std::vector<int32_t> items;     // item_words per work item, see PrefixArgs::items
+    std::vector<int32_t> seqs;      // 8 per sequence, see PrefixArgs::seqs
+    std::vector<int32_t> tiles;     // 2 per row tile: first slot, pieces
     pd_plan *suffix = nullptr;
     pd::PrefixImage image;
     std::vector<uint8_t> host_image;
     uint8_t *dev = nullptr;
-    const void *k = nullptr, *v = nullptr;   // the caches the tensor maps describe
-    alignas(64) CUtensorMap map_k, map_v;
 
     ~pd_prefix_plan() { delete suffix; }
 };

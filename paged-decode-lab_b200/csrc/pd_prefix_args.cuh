@@ -9,9 +9,15 @@ namespace pd {
 struct PrefixArgs {
     const void *q;              // [B, Hq, D]
     const void *k, *v;          // [P, T, Hkv, D]
-    const int4 *items;          // 2 per work item: {first member, members, KV head, tile},
-                                // {first page in `pages`, first and end page of the piece, slot}
-    const int4 *seqs;           // per sequence: {member index or -1, first slot, tiles, pieces} of its group
+    // Work items.  FP32: 2 words of 4: {first member, members, KV head, row tile}, {first of the
+    // group's pages in `pages`, first and end page of the piece, partial slot}.  FP16: 4 of them:
+    // {first member, members, KV head, paired}, {first of the group's pages in `pages`, 0, 0, 0},
+    // and per stream {row tile, first page, end page, slot}.
+    const int4 *items;
+    // Per sequence: {member index in its group or -1, first row tile of KV head 0, row tiles per KV
+    // head, first of the group's pages in `pages`}, {shared pages, 0, 0, 0}.
+    const int4 *seqs;
+    const int2 *tiles;          // per row tile: {first partial slot, pieces}
     const int32_t *members;     // sequences of the groups, one after another
     const int32_t *pages;       // shared pages of the groups, one after another
     const int32_t *lengths;     // [B]

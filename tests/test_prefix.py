@@ -104,8 +104,22 @@ def test_matches_attention_in_64_bits(dtype, heads, kv, D, page, groups, others)
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_long_prefix_split_over_many_ctas(dtype):
     layout, table, lengths, members, q, k, v = case([(700, [0, 33, 5])], [], 8, 2, 128, 16, dtype)
-    out = SharedPrefixPlan(layout, table, lengths, prefixes=members, dtype=dtype).run(q, k, v)
-    close(out, *exact(q, k, v, table, lengths))
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=members, dtype=dtype)
+    close(plan.run(q, k, v), *exact(q, k, v, table, lengths))
+    assert plan.read_errors() == 0
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (64, 32), (128, 16), (128, 32)])
+@pytest.mark.parametrize("tokens", [16384, 12000])
+def test_many_steps_per_cta(D, page, tokens):
+    """Enough tiles that a CTA walks many 128-token steps, in pairs of tiles and (odd tile counts) in halves."""
+    groups = [(tokens // page, list(range(70))), (tokens // 2 // page, [3] * 33)]
+    layout, table, lengths, members, q, k, v = case(groups, [], 64, 8, D, page, F16)
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=members)
+    out = plan.run(q, k, v)
+    some = np.r_[0:103:17]
+    close(out[some], *exact(q[some], k, v, table[some], lengths[some]))
+    assert plan.read_errors() == 0
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
