@@ -9,7 +9,10 @@
 // values are copied bit for bit.
 #include <algorithm>
 #include <cmath>
+#include <mutex>
+#include <set>
 #include <string>
+#include <utility>
 
 #include "paged_decode.h"
 #include "pd_device.cuh"
@@ -40,62 +43,70 @@ struct RotaryArgs {
     // append: k.out and v.out are the caches [P, T, kv_heads, D]
     const int32_t *page_table, *lengths, *indptr;   // [B, W], [B], [B + 1] or NULL (one token per sequence)
     int64_t width, pages;
-    int32_t batch, page_size;
+    int32_t batch, page_shift;                   // log2 of the page size
     uint32_t *error;
 };
 
-constexpr int kRows = 4;              // rows a thread loads before it works on the first
-constexpr int kMaxThreads = 512;
+// The direct kernel: rows that a lane holds at once, and the largest CTA.
+constexpr int kRows = 4, kMaxThreads = 512;
+// The streaming kernel: consumer warps beside one producer warp, CTAs per SM and
+// the shared memory of each one's stages.
+constexpr int kConsumers = 8, kStreamCtas = 3, kStreamThreads = 32 * (kConsumers + 1);
+constexpr int kMaxStages = 8, kMinStages = 3, kRingBytes = 70 * 1024;
 constexpr uint32_t kErrBadPage = PD_DEVERR_BAD_PAGE, kErrLength = PD_DEVERR_LENGTH, kErrPosition = PD_DEVERR_POSITION;
 
+// One thread's part of a row: two pieces of 8 bytes, each moved whole when
+// everything is 8-byte aligned (VECTOR), else element by element.
 template <typename Elt>
-__device__ __forceinline__ float to_float(Elt x) {
-    return float(x);
-}
-template <>
-__device__ __forceinline__ float to_float<__half>(__half x) {
-    return __half2float(x);
-}
-
+struct alignas(8) Piece {
+    static constexpr int H = 8 / int(sizeof(Elt));   // elements
+    Elt e[H];
+};
 template <typename Elt>
-__device__ __forceinline__ Elt from_float(float x);
-template <>
-__device__ __forceinline__ float from_float<float>(float x) {
-    return x;
-}
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) {
-    return __float2half_rn(x);
-}
-
-// One thread's part of a row: 16 bytes, moved whole when everything is
-// 16-byte aligned (VECTOR), else element by element.
-template <typename Elt>
-struct alignas(16) Part {
-    static constexpr int N = 16 / int(sizeof(Elt));
-    Elt e[N];
+struct Part {
+    Piece<Elt> lo, hi;
 };
 
 template <typename Elt, bool VECTOR>
-__device__ __forceinline__ Part<Elt> load_part(const Elt *p) {
-    Part<Elt> r;
+__device__ __forceinline__ void load_piece(Piece<Elt> &r, const Elt *p) {
     if constexpr (VECTOR) {
-        *reinterpret_cast<uint4 *>(&r) = *reinterpret_cast<const uint4 *>(p);
+        *reinterpret_cast<uint2 *>(&r) = *reinterpret_cast<const uint2 *>(p);
     } else {
 #pragma unroll
-        for (int i = 0; i < Part<Elt>::N; ++i) r.e[i] = p[i];
+        for (int i = 0; i < Piece<Elt>::H; ++i) r.e[i] = p[i];
     }
-    return r;
 }
 
 template <typename Elt, bool VECTOR>
-__device__ __forceinline__ void store_part(Elt *p, const Part<Elt> &r) {
+__device__ __forceinline__ void store_piece(Elt *p, const Piece<Elt> &r) {
     if constexpr (VECTOR) {
-        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&r);
+        *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(&r);
     } else {
 #pragma unroll
-        for (int i = 0; i < Part<Elt>::N; ++i) p[i] = r.e[i];
+        for (int i = 0; i < Piece<Elt>::H; ++i) p[i] = r.e[i];
     }
+}
+
+// A piece in FP32, two elements to a register pair, and back (one rounding).
+using f32x2 = unsigned long long;
+__device__ __forceinline__ void widen(f32x2 (&x)[2], const Piece<__half> &p) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&p.e[2 * i]));
+        x[i] = pack_f32x2(v.x, v.y);
+    }
+}
+__device__ __forceinline__ void widen(f32x2 (&x)[1], const Piece<float> &p) { x[0] = pack_f32x2(p.e[0], p.e[1]); }
+__device__ __forceinline__ void narrow(Piece<__half> &p, const f32x2 (&x)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 v = unpack_f32x2(x[i]);
+        *reinterpret_cast<__half2 *>(&p.e[2 * i]) = __floats2half2_rn(v.x, v.y);
+    }
+}
+__device__ __forceinline__ void narrow(Piece<float> &p, const f32x2 (&x)[1]) {
+    const float2 v = unpack_f32x2(x[0]);
+    p.e[0] = v.x, p.e[1] = v.y;
 }
 
 // The sequence of token i: the last b with indptr[b] <= i (a binary search;
@@ -110,190 +121,473 @@ __device__ __forceinline__ int sequence_of(const int32_t *indptr, int batch, int
     return lo;
 }
 
-// One CTA per token (grid-stride).  A row is D / N lanes of one warp, 16 bytes
-// each; a CTA holds blockDim / lanes row slots, and row slot s takes rows s, s
-// + slots, .. of [queries][keys][values].  The first kRows rows of a thread are
-// in flight before it looks up where the token goes.
-template <typename Elt, int D, bool VECTOR, bool APPEND>
-__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const RotaryArgs a) {
-    using P = Part<Elt>;
-    constexpr int N = P::N, LANES = D / N;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int slots = blockDim.x / LANES;
-    const int slot = threadIdx.x / LANES;
-    const int lane = threadIdx.x % LANES;
-    const int e0 = lane * N;                    // first element of this thread's part
-    const int kq = a.q.heads, kk = kq + a.k.heads, rows = kk + a.v.heads;   // ends of queries, keys, values
-    const int half = a.rotary / 2, half_lanes = half / N;
-    const bool turns = a.table && lane < a.rotary / N;
-    const bool first = lane < half_lanes;       // half-split: this thread holds the pairs' first elements
-    // the lane with the pairs' other elements
-    const int mate = (threadIdx.x & 31) + (!turns || a.interleaved ? 0 : first ? half_lanes : -half_lanes);
+// Where a token goes.
+struct Place {
+    int64_t position;
+    int64_t cache_row;      // row (page * T + offset) of the cache
+    bool live;              // false: its query rows are zeros, nothing is appended
+};
 
-    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
-        P part[kRows];
-        const auto load = [&](int base) {
-#pragma unroll
-            for (int u = 0; u < kRows; ++u) {
-                const int row = base + slot + u * slots;
-                if (row >= rows) continue;
-                const bool is_q = row < kq, is_k = row < kk;
-                const void *data = is_q ? a.q.data : is_k ? a.k.data : a.v.data;
-                const int64_t ts = is_q ? a.q.token_stride : is_k ? a.k.token_stride : a.v.token_stride;
-                const int64_t hs = is_q ? a.q.head_stride : is_k ? a.k.head_stride : a.v.head_stride;
-                const int head = row - (is_q ? 0 : is_k ? kq : kk);
-                part[u] = load_part<Elt, VECTOR>(static_cast<const Elt *>(data) + token * ts + head * hs + e0);
-            }
-        };
-        load(0);
-
-        // ---- where the token goes
-        int64_t position, cache_row = 0;        // cache_row: row (page * T + offset) of the cache
-        bool live = true;                       // false: its query rows are zeros, nothing is appended
-        if constexpr (APPEND) {
-            int b;
-            int64_t to_end;                     // tokens from this one to the sequence's end
-            if (a.indptr) {
-                b = sequence_of(a.indptr, a.batch, token);
-                to_end = __ldg(a.indptr + b + 1) - token;   // <= 0: padding past the last sequence
-            } else {
-                b = int(token);
-                to_end = 1;
-            }
-            const int64_t length = __ldg(a.lengths + b);
-            position = length - to_end;
-            if (to_end <= 0 || (!a.indptr && length == 0)) {
-                live = false;                   // padding, or a sequence that is not in use
-            } else if (position < 0 || position >= a.width * a.page_size) {
-                live = false;
-                if (threadIdx.x == 0) atomicOr(a.error, kErrLength);
-            } else {
-                const int32_t page = __ldg(a.page_table + int64_t(b) * a.width + position / a.page_size);
-                if (page >= 0 && page < a.pages) {
-                    cache_row = int64_t(page) * a.page_size + position % a.page_size;
-                } else {
-                    live = false;
-                    if (threadIdx.x == 0) atomicOr(a.error, kErrBadPage);
-                }
-            }
+// `report`: this thread flags a token that is skipped.
+template <bool APPEND>
+__device__ __forceinline__ Place place_of(const RotaryArgs &a, int64_t token, bool report) {
+    Place p{0, 0, true};
+    uint32_t flag = 0;
+    if constexpr (APPEND) {
+        int b;
+        int64_t to_end;     // tokens from this one to the sequence's end
+        if (a.indptr) {
+            b = sequence_of(a.indptr, a.batch, token);
+            to_end = __ldg(a.indptr + b + 1) - token;   // <= 0: padding past the last sequence
         } else {
-            position = __ldg(a.positions + token);
+            b = int(token);
+            to_end = 1;
         }
-        if (live && a.table && (position < 0 || position >= a.max_positions)) {
-            live = false;
-            if (threadIdx.x == 0) atomicOr(a.error, kErrPosition);
+        const int64_t length = __ldg(a.lengths + b);
+        p.position = length - to_end;
+        if (to_end <= 0 || (!a.indptr && length == 0)) {
+            p.live = false;                             // padding, or a sequence that is not in use
+        } else if (p.position < 0 || p.position >= (a.width << a.page_shift)) {
+            flag = kErrLength;
+        } else {
+            const int at = int(p.position);
+            const int32_t page = __ldg(a.page_table + int64_t(b) * a.width + (at >> a.page_shift));
+            if (page >= 0 && page < a.pages)
+                p.cache_row = (int64_t(page) << a.page_shift) + (at & ((1 << a.page_shift) - 1));
+            else flag = kErrBadPage;
         }
-        float c[N], s[N];                       // cos and sin of the thread's pairs (interleaved: the first N / 2)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            c[i] = 1.f;
-            s[i] = 0.f;
-        }
-        if (turns && live) {
-            const float *t = a.table + position * a.rotary + (a.interleaved ? e0 / 2 : first ? e0 : e0 - half);
-#pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                if (a.interleaved && i >= N / 2) continue;
-                const float2 cc = __ldg(reinterpret_cast<const float2 *>(t + i));
-                const float2 ss = __ldg(reinterpret_cast<const float2 *>(t + half + i));
-                c[i] = cc.x, c[i + 1] = cc.y;
-                s[i] = ss.x, s[i + 1] = ss.y;
-            }
-        }
+    } else {
+        p.position = __ldg(a.positions + token);
+    }
+    if (p.live && !flag && a.table && (p.position < 0 || p.position >= a.max_positions)) flag = kErrPosition;
+    if (flag) {
+        p.live = false;
+        if (report) atomicOr(a.error, flag);
+    }
+    return p;
+}
 
-        for (int base = 0;;) {
+// The cosines and sines of a lane's pairs, as its two pieces x and y meet them:
+//   half-split    x' = x c + y t, y' = y c + x t2        with t = -s, t2 = s
+//   interleaved   x' = x c + swap(x) t, y' = y c2 + swap(y) t2   with (c, c), (-s, s) per pair
+template <int W>
+struct Turn {
+    f32x2 c[W], t[W], c2[W], t2[W];
+};
+
+// From the table's cosines and sines of the lane's H = 2 W pairs.
+template <int W, bool INTERLEAVED>
+__device__ __forceinline__ void load_turn(Turn<W> &r, const float *c, const float *s) {
+    float cc[2 * W], ss[2 * W];
 #pragma unroll
-            for (int u = 0; u < kRows; ++u) {
-                // The row's lanes are neighbours in one warp, whose other rows may be of another
-                // kind or past the end: every lane takes part in the exchanges.
-                const int row = base + slot + u * slots;
-                const bool is_q = row < kq, is_k = !is_q && row < kk;
-                const float *weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
-                float x[N];
+    for (int i = 0; i < W; ++i) {
+        const float2 x = *reinterpret_cast<const float2 *>(c + 2 * i), y = *reinterpret_cast<const float2 *>(s + 2 * i);
+        cc[2 * i] = x.x, cc[2 * i + 1] = x.y;
+        ss[2 * i] = y.x, ss[2 * i + 1] = y.y;
+    }
 #pragma unroll
-                for (int i = 0; i < N; ++i) x[i] = row < rows ? to_float<Elt>(part[u].e[i]) : 0.f;
-                if (a.q_weight || a.k_weight) {
-                    float sum = 0.f;
-#pragma unroll
-                    for (int i = 0; i < N; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-                    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-                    if (weight) {
-                        const float scale = rsqrtf(sum / float(D) + a.eps);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) x[i] = x[i] * scale * __ldg(weight + e0 + i);
-                    }
-                }
-                if (a.table) {
-                    if (a.interleaved) {
-                        if (turns) {
-#pragma unroll
-                            for (int i = 0; i < N; i += 2) {
-                                const float p = x[i], q = x[i + 1];
-                                x[i] = fmaf(p, c[i / 2], -q * s[i / 2]);
-                                x[i + 1] = fmaf(q, c[i / 2], p * s[i / 2]);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const float m = __shfl_sync(kFullMask, x[i], mate);
-                            if (turns) x[i] = fmaf(x[i], c[i], first ? -m * s[i] : m * s[i]);
-                        }
-                    }
-                }
-                if (row >= rows) continue;
-                P r = part[u];                  // values stay as they are
-                if (is_q || is_k) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) r.e[i] = from_float<Elt>(live ? x[i] : 0.f);
-                }
-                Elt *dst;
-                if (is_q) {
-                    dst = static_cast<Elt *>(a.q.out) + token * a.q.out_token_stride + row * a.q.out_head_stride;
-                } else if constexpr (APPEND) {
-                    if (!live) continue;
-                    dst = static_cast<Elt *>(is_k ? a.k.out : a.v.out) +
-                          (cache_row * a.k.heads + (row - (is_k ? kq : kk))) * D;
-                } else {
-                    dst = static_cast<Elt *>(a.k.out) + token * a.k.out_token_stride + (row - kq) * a.k.out_head_stride;
-                }
-                store_part<Elt, VECTOR>(dst + e0, r);
-            }
-            base += slots * kRows;
-            if (base >= rows) break;
-            load(base);
+    for (int i = 0; i < W; ++i) {
+        if (INTERLEAVED) {      // pair i in x, pair W + i in y
+            r.c[i] = pack_f32x2(cc[i], cc[i]);
+            r.t[i] = pack_f32x2(-ss[i], ss[i]);
+            r.c2[i] = pack_f32x2(cc[W + i], cc[W + i]);
+            r.t2[i] = pack_f32x2(-ss[W + i], ss[W + i]);
+        } else {
+            r.c[i] = pack_f32x2(cc[2 * i], cc[2 * i + 1]);
+            r.t[i] = pack_f32x2(-ss[2 * i], -ss[2 * i + 1]);
+            r.t2[i] = pack_f32x2(ss[2 * i], ss[2 * i + 1]);
         }
     }
 }
 
-template <typename Elt, int D>
-cudaError_t launch_rotary(const RotaryArgs &a, bool vector, bool append, cudaStream_t stream) {
-    constexpr int LANES = D * int(sizeof(Elt)) / 16;
-    const int rows = a.q.heads + a.k.heads + a.v.heads;
-    // row slots: a thread's kRows rows cover the token, in whole warps
-    int threads = (rows + kRows - 1) / kRows * LANES;
-    threads = std::min(kMaxThreads, (threads + 31) / 32 * 32);
+// 2 W floats from 8-byte aligned memory.
+template <int W>
+__device__ __forceinline__ void load_floats(f32x2 (&r)[W], const float *p) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] = *reinterpret_cast<const f32x2 *>(p + 2 * i);
+}
+
+// One lane's part of a row: the norm, then the rotation.  With `sums` every lane
+// of the warp takes part in its rows' sums; `norms`: this row uses them.
+template <typename Elt, int LANES, bool INTERLEAVED>
+__device__ __forceinline__ void norm_rotate(Part<Elt> &part, bool sums, bool norms, const f32x2 (&wlo)[Piece<Elt>::H / 2],
+                                            const f32x2 (&whi)[Piece<Elt>::H / 2], float eps, bool turns,
+                                            const Turn<Piece<Elt>::H / 2> &r) {
+    constexpr int W = Piece<Elt>::H / 2;
+    f32x2 x[W], y[W];
+    widen(x, part.lo);
+    widen(y, part.hi);
+    if (sums) {
+        f32x2 sum2 = mul_f32x2(x[0], x[0]);
+#pragma unroll
+        for (int i = 1; i < W; ++i) sum2 = fma_f32x2(x[i], x[i], sum2);
+#pragma unroll
+        for (int i = 0; i < W; ++i) sum2 = fma_f32x2(y[i], y[i], sum2);
+        float sum = unpack_f32x2(sum2).x + unpack_f32x2(sum2).y;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        if (norms) {
+            const float scale = rsqrtf(fmaf(sum, 1.f / float(LANES * 4 * W), eps));
+            const f32x2 scale2 = pack_f32x2(scale, scale);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                x[i] = mul_f32x2(x[i], mul_f32x2(wlo[i], scale2));
+                y[i] = mul_f32x2(y[i], mul_f32x2(whi[i], scale2));
+            }
+        }
+    }
+    if (turns) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (INTERLEAVED) {
+                const float2 u = unpack_f32x2(x[i]), v = unpack_f32x2(y[i]);
+                x[i] = fma_f32x2(x[i], r.c[i], mul_f32x2(pack_f32x2(u.y, u.x), r.t[i]));
+                y[i] = fma_f32x2(y[i], r.c2[i], mul_f32x2(pack_f32x2(v.y, v.x), r.t2[i]));
+            } else {
+                const f32x2 u = mul_f32x2(y[i], r.t[i]), v = mul_f32x2(x[i], r.t2[i]);
+                x[i] = fma_f32x2(x[i], r.c[i], u);
+                y[i] = fma_f32x2(y[i], r.c[i], v);
+            }
+        }
+    }
+    narrow(part.lo, x);
+    narrow(part.hi, y);
+}
+
+// A row is D / N lanes of one warp.  A lane holds both elements of each of its
+// pairs, so that the rotation needs no exchange and half the cosines: pieces
+// [H lane, +H) and r/2 further on in half-split rows, neighbouring pieces in
+// interleaved ones and past the rotation.
+template <typename Elt, int D, bool INTERLEAVED>
+struct Lane {
+    static constexpr int H = Piece<Elt>::H, W = H / 2, N = 2 * H, LANES = D / N, PER_WARP = 32 / LANES;
+    int lane, lo, hi;
+    bool turns;
+    __device__ __forceinline__ explicit Lane(const RotaryArgs &a) {
+        lane = threadIdx.x % LANES;
+        turns = lane < a.rotary / N;
+        const bool apart = turns && !INTERLEAVED;
+        lo = apart ? H * lane : N * lane;
+        hi = apart ? lo + a.rotary / 2 : lo + H;
+    }
+};
+
+// Direct kernel: any strides and alignment, few tokens.  One CTA per token; its
+// row slots take rows slot, slot + slots, .. of [queries][keys][values], kRows of
+// them in flight before the token's place is looked up.
+template <typename Elt, int D, bool VECTOR, bool APPEND, bool INTERLEAVED>
+__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const RotaryArgs a) {
+    using P = Part<Elt>;
+    using L = Lane<Elt, D, INTERLEAVED>;
+    constexpr int H = L::H, W = L::W, LANES = L::LANES;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const L l(a);
+    const int slots = blockDim.x / LANES, slot = threadIdx.x / LANES;
+    const int kq = a.q.heads, kk = kq + a.k.heads, rows = kk + a.v.heads;   // ends of queries, keys, values
+    const int64_t token = blockIdx.x;
+    P part[kRows];
+    const auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int row = base + slot + u * slots;
+            if (row >= rows) continue;
+            const bool is_q = row < kq, is_k = row < kk;
+            const Elt *p = static_cast<const Elt *>(is_q ? a.q.data : is_k ? a.k.data : a.v.data);
+            const int64_t ts = is_q ? a.q.token_stride : is_k ? a.k.token_stride : a.v.token_stride;
+            const int64_t hs = is_q ? a.q.head_stride : is_k ? a.k.head_stride : a.v.head_stride;
+            p += token * ts + (row - (is_q ? 0 : is_k ? kq : kk)) * hs;
+            load_piece<Elt, VECTOR>(part[u].lo, p + l.lo);
+            load_piece<Elt, VECTOR>(part[u].hi, p + l.hi);
+        }
+    };
+    load(0);
+    const Place at = place_of<APPEND>(a, token, threadIdx.x == 0);
+    Turn<W> turn;
+    if (l.turns && at.live) {
+        const float *t = a.table + at.position * a.rotary + H * l.lane;
+        load_turn<W, INTERLEAVED>(turn, t, t + a.rotary / 2);
+    }
+    for (int base = 0;;) {
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int row = base + slot + u * slots;
+            const bool is_q = row < kq, is_k = !is_q && row < kk;
+            if (__any_sync(kFullMask, is_q || is_k)) {
+                f32x2 wlo[W], whi[W];
+                Part<Elt> r = part[u];
+                const float *weight = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
+                if (weight) {
+                    load_floats<W>(wlo, weight + l.lo);
+                    load_floats<W>(whi, weight + l.hi);
+                }
+                norm_rotate<Elt, LANES, INTERLEAVED>(r, a.q_weight || a.k_weight, weight != nullptr, wlo, whi, a.eps,
+                                                     l.turns && at.live, turn);
+                if (is_q || is_k) part[u] = at.live ? r : Part<Elt>{};      // values stay as they are
+            }
+            if (row >= rows) continue;
+            Elt *dst;
+            if (is_q) {
+                dst = static_cast<Elt *>(a.q.out) + token * a.q.out_token_stride + row * a.q.out_head_stride;
+            } else if constexpr (APPEND) {
+                if (!at.live) continue;
+                dst = static_cast<Elt *>(is_k ? a.k.out : a.v.out) +
+                      (at.cache_row * a.k.heads + (row - (is_k ? kq : kk))) * D;
+            } else {
+                dst = static_cast<Elt *>(a.k.out) + token * a.k.out_token_stride + (row - kq) * a.k.out_head_stride;
+            }
+            store_piece<Elt, VECTOR>(dst + l.lo, part[u].lo);
+            store_piece<Elt, VECTOR>(dst + l.hi, part[u].hi);
+        }
+        base += slots * kRows;
+        if (base >= rows) break;
+        load(base);
+    }
+}
+
+// ---------------------------------------------------------------- streaming kernel
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+// Shared memory: [stages][q | k | v | table row] barriers.
+struct StreamShape {
+    int q_bytes, k_bytes, v_bytes, stage_bytes, stages;
+    size_t smem;
+};
+
+// Streaming kernel: many tokens whose rows lie one after another (16-byte
+// aligned).  A persistent CTA takes every gridDim-th token through a ring of
+// stages: the producer warp brings a token's queries, keys, values and its
+// row of the rotation table by bulk copies, the consumer warps norm and rotate
+// the rows where they are, and the producer sends the whole token on by bulk
+// stores.  Places are looked up by the producer's lanes, 32 tokens at a time.
+template <typename Elt, int D, bool APPEND, bool INTERLEAVED>
+__global__ void __launch_bounds__(kStreamThreads, kStreamCtas) rotary_stream_kernel(const RotaryArgs a, const StreamShape sh) {
+    using L = Lane<Elt, D, INTERLEAVED>;
+    constexpr int H = L::H, W = L::W, LANES = L::LANES, PER_WARP = L::PER_WARP;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + size_t(sh.stages) * sh.stage_bytes);
+    uint64_t *done = full + kMaxStages;
+    int64_t *cache_rows = reinterpret_cast<int64_t *>(done + kMaxStages);
+    volatile int *lives = reinterpret_cast<volatile int *>(cache_rows + kMaxStages);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stages = sh.stages;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; ++i) {
+            mbar_init(smem_u32(full + i), 1);
+            mbar_init(smem_u32(done + i), kConsumers);
+        }
+        mbar_init_fence();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __syncthreads();
+    // this CTA's tokens; tokens fit 31 bits
+    const int n = (int(a.tokens) - int(blockIdx.x) + int(gridDim.x) - 1) / int(gridDim.x);
+    const auto token_of = [&](int j) { return blockIdx.x + int64_t(j) * gridDim.x; };
+    // token j is in stage j % stages, whose barriers are then in phase j / stages
+    struct Turnstile {
+        int stage = 0, phase = 0;
+        __device__ __forceinline__ void next(int stages) {
+            if (++stage == stages) stage = 0, phase ^= 1;
+        }
+    };
+
+    if (warp == kConsumers) {
+        Place batch{};
+        int loaded = 0;                 // tokens whose loads were issued
+        int load_stage = 0;
+        const auto load = [&]() {       // the next token's
+            const int j = loaded++, st = load_stage;
+            if (++load_stage == stages) load_stage = 0;
+            if ((j & 31) == 0 && j + lane < n) batch = place_of<APPEND>(a, token_of(j + lane), true);
+            const int from = j & 31;
+            const int64_t position = __shfl_sync(kFullMask, batch.position, from);
+            const int64_t cache_row = __shfl_sync(kFullMask, batch.cache_row, from);
+            const bool live = __shfl_sync(kFullMask, int(batch.live), from) != 0;
+            if (lane != 0) return;
+            cache_rows[st] = cache_row;
+            lives[st] = live;
+            const uint32_t bar = smem_u32(full + st), dst = smem_u32(smem + size_t(st) * sh.stage_bytes);
+            const int turn_bytes = a.table && live ? a.rotary * 4 : 0;
+            mbar_arrive_expect_tx(bar, uint32_t(sh.q_bytes + sh.k_bytes + sh.v_bytes + turn_bytes));
+            const int64_t token = token_of(j);
+            if (sh.q_bytes) bulk_load(dst, static_cast<const Elt *>(a.q.data) + token * a.q.token_stride, sh.q_bytes, bar);
+            if (sh.k_bytes)
+                bulk_load(dst + sh.q_bytes, static_cast<const Elt *>(a.k.data) + token * a.k.token_stride, sh.k_bytes, bar);
+            if (sh.v_bytes)
+                bulk_load(dst + sh.q_bytes + sh.k_bytes, static_cast<const Elt *>(a.v.data) + token * a.v.token_stride,
+                          sh.v_bytes, bar);
+            if (turn_bytes)
+                bulk_load(dst + sh.q_bytes + sh.k_bytes + sh.v_bytes, a.table + position * a.rotary, turn_bytes, bar);
+        };
+        while (loaded < min(n, stages)) load();
+        Turnstile at;
+        for (int j = 0; j < n; ++j, at.next(stages)) {
+            const int st = at.stage;
+            if (!__all_sync(kFullMask, mbar_wait(smem_u32(done + st), at.phase))) {
+                if (lane == 0) atomicOr(a.error, PD_DEVERR_TIMEOUT);
+                break;
+            }
+            if (lane == 0) {
+                const int64_t token = token_of(j);
+                const uint32_t src = smem_u32(smem + size_t(st) * sh.stage_bytes);
+                if (sh.q_bytes) bulk_store(static_cast<Elt *>(a.q.out) + token * a.q.out_token_stride, src, sh.q_bytes);
+                if constexpr (APPEND) {
+                    if (lives[st]) {
+                        const int64_t at = cache_rows[st] * a.k.heads * D;
+                        bulk_store(static_cast<Elt *>(a.k.out) + at, src + sh.q_bytes, sh.k_bytes);
+                        bulk_store(static_cast<Elt *>(a.v.out) + at, src + sh.q_bytes + sh.k_bytes, sh.v_bytes);
+                    }
+                } else if (sh.k_bytes) {
+                    bulk_store(static_cast<Elt *>(a.k.out) + token * a.k.out_token_stride, src + sh.q_bytes, sh.k_bytes);
+                }
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                // all but the newest store have read their stages: token j - 1's is free
+                asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            }
+            __syncwarp();
+            if (j > 0 && loaded < n) load();
+        }
+        // no copy is in flight when the CTA ends
+        for (int j = max(0, loaded - stages); j < loaded; ++j)
+            if (!mbar_wait(smem_u32(full + j % stages), (j / stages) & 1) && lane == 0) atomicOr(a.error, PD_DEVERR_TIMEOUT);
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else {
+        const L l(a);
+        f32x2 q_lo[W], q_hi[W], k_lo[W], k_hi[W];
+        if (a.q_weight) {
+            load_floats<W>(q_lo, a.q_weight + l.lo);
+            load_floats<W>(q_hi, a.q_weight + l.hi);
+        }
+        if (a.k_weight) {
+            load_floats<W>(k_lo, a.k_weight + l.lo);
+            load_floats<W>(k_hi, a.k_weight + l.hi);
+        }
+        Turnstile at;
+        for (int j = 0; j < n; ++j, at.next(stages)) {
+            const int st = at.stage;
+            if (!__all_sync(kFullMask, mbar_wait(smem_u32(full + st), at.phase))) {
+                if (lane == 0) atomicOr(a.error, PD_DEVERR_TIMEOUT);
+                break;
+            }
+            uint8_t *stage = smem + size_t(st) * sh.stage_bytes;
+            const bool live = lives[st] != 0;
+            Turn<W> turn;
+            if (l.turns) {
+                const float *t = reinterpret_cast<const float *>(stage + sh.q_bytes + sh.k_bytes + sh.v_bytes) + H * l.lane;
+                load_turn<W, INTERLEAVED>(turn, t, t + a.rotary / 2);
+            }
+            // rows of one kind: PER_WARP for each warp at a time, beginning with warp `first`
+            const auto work = [&](Elt *rows, int heads, int first, bool norms, const f32x2 (&lo)[W], const f32x2 (&hi)[W]) {
+                if (!norms && !a.table && live) return;
+                for (int base = first * PER_WARP; base < heads; base += kConsumers * PER_WARP) {
+                    const int row = base + lane / LANES;
+                    Elt *x = rows + row * D;
+                    Part<Elt> part{};
+                    if (row < heads) {
+                        load_piece<Elt, true>(part.lo, x + l.lo);
+                        load_piece<Elt, true>(part.hi, x + l.hi);
+                    }
+                    norm_rotate<Elt, LANES, INTERLEAVED>(part, norms, norms, lo, hi, a.eps, l.turns, turn);
+                    if (!live) part = Part<Elt>{};
+                    if (row < heads) {
+                        store_piece<Elt, true>(x + l.lo, part.lo);
+                        store_piece<Elt, true>(x + l.hi, part.hi);
+                    }
+                }
+            };
+            work(reinterpret_cast<Elt *>(stage), a.q.heads, warp, a.q_weight != nullptr, q_lo, q_hi);
+            work(reinterpret_cast<Elt *>(stage + sh.q_bytes), a.k.heads, kConsumers - 1 - warp, a.k_weight != nullptr, k_lo,
+                 k_hi);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // before the bulk stores read it
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(done + st));
+        }
+    }
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, size_t smem, cudaStream_t stream,
+                             const Args &...args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(std::min<int64_t>(a.tokens, 1 << 30)));
+    cfg.gridDim = dim3(unsigned(grid));
     cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (append)
-        return vector ? cudaLaunchKernelEx(&cfg, rotary_kernel<Elt, D, true, true>, a)
-                      : cudaLaunchKernelEx(&cfg, rotary_kernel<Elt, D, false, true>, a);
-    return vector ? cudaLaunchKernelEx(&cfg, rotary_kernel<Elt, D, true, false>, a)
-                  : cudaLaunchKernelEx(&cfg, rotary_kernel<Elt, D, false, false>, a);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Rows, strides and pointers of one operand; `vector` turns false when its
-// parts are not 16-byte aligned.
-pd_status check_rows(const pd_heads *h, const char *name, int elt, bool needs_out, bool *vector, HeadRows *rows) {
+// The streaming kernels whose dynamic shared memory was raised, per device.
+std::mutex g_stream_mutex;
+std::set<std::pair<int, const void *>> g_stream_done;
+
+cudaError_t allow_stream_smem(int device, const void *kernel) {
+    std::lock_guard<std::mutex> lock(g_stream_mutex);
+    if (g_stream_done.count({device, kernel})) return cudaSuccess;
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 4096);
+    if (err == cudaSuccess) g_stream_done.insert({device, kernel});
+    return err;
+}
+
+// What a call's operands allow: whole 8-byte pieces, whole 16-byte aligned rows one after another.
+struct Alignment {
+    bool pieces = true, rows = true;
+};
+
+template <typename Elt, int D, bool APPEND, bool INTERLEAVED>
+cudaError_t launch_rotary(const RotaryArgs &a, Alignment align, int device, cudaStream_t stream) {
+    constexpr int LANES = D * int(sizeof(Elt)) / 16;
+    int sms = 148;
+    cudaError_t err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (err != cudaSuccess) return err;
+    // Streaming pays when each of its CTAs has several tokens to overlap.
+    StreamShape sh{};
+    const int row = D * int(sizeof(Elt));
+    const int64_t token_bytes = int64_t(a.q.heads + a.k.heads + a.v.heads) * row + a.rotary * 4;
+    if (align.rows && a.tokens >= int64_t(kStreamCtas) * sms * kMinStages && token_bytes * kMinStages <= kRingBytes) {
+        sh.q_bytes = a.q.heads * row;
+        sh.k_bytes = a.k.heads * row;
+        sh.v_bytes = a.v.heads * row;
+        sh.stage_bytes = int((token_bytes + 127) / 128 * 128);
+        sh.stages = std::min(kMaxStages, kRingBytes / sh.stage_bytes);
+        sh.smem = size_t(sh.stages) * sh.stage_bytes + kMaxStages * (8 + 8 + 8 + 4);
+        const auto kernel = rotary_stream_kernel<Elt, D, APPEND, INTERLEAVED>;
+        err = allow_stream_smem(device, reinterpret_cast<const void *>(kernel));
+        if (err != cudaSuccess) return err;
+        return launch_dependent(kernel, std::min<int64_t>(a.tokens, int64_t(kStreamCtas) * sms), kStreamThreads, sh.smem,
+                                stream, a, sh);
+    }
+    // row slots: a thread's kRows rows cover the token, in whole warps
+    const int rows = a.q.heads + a.k.heads + a.v.heads;
+    int threads = (rows + kRows - 1) / kRows * LANES;
+    threads = std::min(kMaxThreads, (threads + 31) / 32 * 32);
+    const auto kernel = align.pieces ? rotary_kernel<Elt, D, true, APPEND, INTERLEAVED>
+                                     : rotary_kernel<Elt, D, false, APPEND, INTERLEAVED>;
+    return launch_dependent(kernel, a.tokens, threads, 0, stream, a);
+}
+
+template <typename Elt, int D>
+cudaError_t launch_rotary(const RotaryArgs &a, Alignment align, bool append, int device, cudaStream_t stream) {
+    const auto launch = append ? (a.interleaved ? launch_rotary<Elt, D, true, true> : launch_rotary<Elt, D, true, false>)
+                               : (a.interleaved ? launch_rotary<Elt, D, false, true> : launch_rotary<Elt, D, false, false>);
+    return launch(a, align, device, stream);
+}
+
+// Rows, strides and pointers of one operand, and what they allow.
+pd_status check_rows(const pd_heads *h, const char *name, int elt, int head_dim, bool needs_out, Alignment *align,
+                     HeadRows *rows) {
     *rows = HeadRows{};
     if (!h) return PD_OK;
     if (h->heads < 0 || h->heads > 65535) return fail(PD_ERR_VALUE, std::string(name) + ": heads must be in [0, 65535]");
@@ -303,7 +597,9 @@ pd_status check_rows(const pd_heads *h, const char *name, int elt, bool needs_ou
     if (at & uintptr_t(elt - 1)) return fail(PD_ERR_VALUE, std::string(name) + " must be aligned to its element size");
     int64_t strides = h->token_stride | h->head_stride;
     if (needs_out) strides |= h->out_token_stride | h->out_head_stride;
-    if ((at & 15) || ((strides * elt) & 15)) *vector = false;
+    if ((at & 7) || ((strides * elt) & 7)) align->pieces = false;
+    if ((at & 15) || ((strides * elt) & 15) || h->head_stride != head_dim || (needs_out && h->out_head_stride != head_dim))
+        align->rows = false;
     *rows = HeadRows{h->data, h->out, h->token_stride, h->head_stride, h->out_token_stride, h->out_head_stride, h->heads};
     return PD_OK;
 }
@@ -330,8 +626,9 @@ pd_status check_rotation(const pd_rotation *r, int head_dim, RotaryArgs *a) {
     return PD_OK;
 }
 
-pd_status run_rotary(const RotaryArgs &a, int head_dim, pd_dtype dtype, bool vector, bool append, int32_t device,
+pd_status run_rotary(const RotaryArgs &a, int head_dim, pd_dtype dtype, Alignment align, bool append, int32_t device,
                      void *stream) {
+    if (a.tokens > INT32_MAX) return fail(PD_ERR_VALUE, "too many tokens");
     if (a.tokens == 0 || a.q.heads + a.k.heads + a.v.heads == 0) return PD_OK;
     int prev = -1;
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
@@ -339,11 +636,11 @@ pd_status run_rotary(const RotaryArgs &a, int head_dim, pd_dtype dtype, bool vec
     if (err != cudaSuccess) return fail(PD_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(err));
     const auto st = static_cast<cudaStream_t>(stream);
     if (dtype == PD_FLOAT16)
-        err = head_dim == 64 ? launch_rotary<__half, 64>(a, vector, append, st)
-                             : launch_rotary<__half, 128>(a, vector, append, st);
+        err = head_dim == 64 ? launch_rotary<__half, 64>(a, align, append, device, st)
+                             : launch_rotary<__half, 128>(a, align, append, device, st);
     else
-        err = head_dim == 64 ? launch_rotary<float, 64>(a, vector, append, st)
-                             : launch_rotary<float, 128>(a, vector, append, st);
+        err = head_dim == 64 ? launch_rotary<float, 64>(a, align, append, device, st)
+                             : launch_rotary<float, 128>(a, align, append, device, st);
     if (prev >= 0 && prev != device) cudaSetDevice(prev);
     if (err != cudaSuccess) return fail(PD_ERR_CUDA, std::string("rotary launch: ") + cudaGetErrorString(err));
     return PD_OK;
@@ -372,16 +669,16 @@ PD_API pd_status pd_rotate_heads(const pd_rotation *rotation, const pd_heads *q,
     RotaryArgs a{};
     if ((s = check_rotation(rotation, rotation->head_dim, &a)) != PD_OK) return s;
     const int elt = dtype == PD_FLOAT16 ? 2 : 4;
-    bool vector = true;
+    Alignment align;
     if (tokens == 0) return PD_OK;
-    if ((s = check_rows(q, "q", elt, true, &vector, &a.q)) != PD_OK) return s;
-    if ((s = check_rows(k, "k", elt, true, &vector, &a.k)) != PD_OK) return s;
+    if ((s = check_rows(q, "q", elt, rotation->head_dim, true, &align, &a.q)) != PD_OK) return s;
+    if ((s = check_rows(k, "k", elt, rotation->head_dim, true, &align, &a.k)) != PD_OK) return s;
     if (!positions || (reinterpret_cast<uintptr_t>(positions) & 3))
         return fail(PD_ERR_VALUE, "positions must be a 4-byte aligned device pointer");
     a.tokens = tokens;
     a.positions = positions;
     a.error = error;
-    return run_rotary(a, rotation->head_dim, dtype, vector, false, device, stream);
+    return run_rotary(a, rotation->head_dim, dtype, align, false, device, stream);
 }
 
 PD_API pd_status pd_cache_append(const pd_layout *layout, const pd_rotation *rotation, const pd_heads *q,
@@ -403,10 +700,10 @@ PD_API pd_status pd_cache_append(const pd_layout *layout, const pd_rotation *rot
     if (table_width < 1 || table_width > INT32_MAX) return fail(PD_ERR_VALUE, "page table must have at least one column");
     if (tokens == 0) return PD_OK;
     const int elt = dtype == PD_FLOAT16 ? 2 : 4;
-    bool vector = true;
-    if ((s = check_rows(q, "q", elt, true, &vector, &a.q)) != PD_OK) return s;
-    if ((s = check_rows(k, "k", elt, false, &vector, &a.k)) != PD_OK) return s;
-    if ((s = check_rows(v, "v", elt, false, &vector, &a.v)) != PD_OK) return s;
+    Alignment align;
+    if ((s = check_rows(q, "q", elt, L.head_dim, true, &align, &a.q)) != PD_OK) return s;
+    if ((s = check_rows(k, "k", elt, L.head_dim, false, &align, &a.k)) != PD_OK) return s;
+    if ((s = check_rows(v, "v", elt, L.head_dim, false, &align, &a.v)) != PD_OK) return s;
     if (!k_cache || !v_cache || !table || !lengths) return fail(PD_ERR_VALUE, "pointers must not be NULL");
     if ((reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache)) & 15)
         return fail(PD_ERR_VALUE, "k_cache and v_cache must be 16-byte aligned");
@@ -421,7 +718,7 @@ PD_API pd_status pd_cache_append(const pd_layout *layout, const pd_rotation *rot
     a.width = table_width;
     a.pages = L.physical_pages;
     a.batch = L.batch;
-    a.page_size = L.page_size;
+    a.page_shift = L.page_size == 16 ? 4 : 5;
     a.error = error;
-    return run_rotary(a, L.head_dim, dtype, vector, true, device, stream);
+    return run_rotary(a, L.head_dim, dtype, align, true, device, stream);
 }

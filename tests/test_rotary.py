@@ -95,6 +95,33 @@ def test_rotate_matches_the_formula(dtype, D, rotary, interleaved, form, heads, 
     assert torch.equal(q, q_out) and torch.equal(k, k_out)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,heads,kv,rotary,interleaved", [(128, 32, 8, 128, False), (128, 5, 1, 32, True),
+                                                           (64, 33, 33, 64, True), (64, 4, 0, 16, False)])
+@pytest.mark.parametrize("tokens", [900, 4099])
+def test_rotate_many_tokens(dtype, D, heads, kv, rotary, interleaved, tokens):
+    """Enough tokens for a persistent grid; the same bits as a few tokens at a time, and as strided heads."""
+    q, k, _ = packed(tokens, heads, kv, D, dtype, "packed")
+    k = k if kv else None
+    qw, kw = weights(D, dtype)
+    op = HeadRotation(D, rotation_table(300, rotary), interleaved=interleaved, q_weight=qw, k_weight=kw if kv != 1 else None)
+    positions = torch.randint(0, 300, (tokens,), device="cuda", dtype=torch.int32)
+    positions[[3, tokens - 2]] = 300                 # outside the table
+    got = op.run(q, k, positions)
+    assert op.read_errors() == POSITION
+    for x, y, w in zip((q, k), got, (qw, kw if kv != 1 else None)):
+        if x is not None:
+            live = positions < 300
+            close(y[live], *exact(x[live], w, positions[live], op.table, interleaved))
+            assert not y[~live].any()
+    few = [op.run(q[i:i + 50], None if k is None else k[i:i + 50], positions[i:i + 50]) for i in range(0, tokens, 50)]
+    swapped = op.run(q.transpose(0, 1).contiguous().transpose(0, 1), k, positions)
+    for i in range(1 + (k is not None)):
+        assert torch.equal(got[i], torch.cat([f[i] for f in few])) and torch.equal(got[i], swapped[i])
+    op.run(q, k, positions, q_out=q, k_out=k)
+    assert torch.equal(q, got[0]) and (k is None or torch.equal(k, got[1]))
+
+
 def test_rotation_table_is_exact_to_fp32():
     t = rotation_table(131072, 128, base=500000.0)
     p, i = 131071, 1
@@ -194,6 +221,39 @@ def test_append_matches_the_formula(dtype, D, page, heads, kv, form, lengths, co
     assert torch.equal(vc[pg, off], v[i])
     kc[pg, off], vc[pg, off] = before[0][pg, off], before[1][pg, off]
     assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])      # nothing else was touched
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,page,heads,kv", [(128, 16, 32, 8), (64, 32, 4, 4), (128, 32, 6, 1)])
+@pytest.mark.parametrize("with_q", [True, False])
+def test_append_many_tokens(dtype, D, page, heads, kv, with_q):
+    """A long ragged prompt batch with padding behind it, a page that is missing and a sequence that is too long."""
+    counts = [700, 0, 1, 333, 64, 1025]
+    lengths = [700, 5, 900, 400, 64, 1030]
+    tokens, padded = sum(counts), sum(counts) + 19
+    table, (kc, vc) = cache_case(lengths, page, kv, D, dtype)
+    table[3, 200 // page] = -1                       # positions of one page of sequence 3
+    q, k, v = packed(padded, heads, kv, D, dtype, "packed", seed=3)
+    rope = rotation_table(1029, D)                   # the last position of sequence 5 is outside
+    qw, kw = weights(D, dtype)
+    op = CacheAppend(Layout(6, heads, kv, D, page, kc.shape[0]), HeadRotation(D, rope, q_weight=qw, k_weight=kw))
+    before = kc.clone(), vc.clone()
+    out = op.run(k, v, kc, vc, torch.tensor(table, device="cuda"),
+                 torch.tensor(lengths, device="cuda", dtype=torch.int32), q=q if with_q else None,
+                 indptr=torch.tensor(np.concatenate(([0], np.cumsum(counts))), device="cuda", dtype=torch.int32))
+    assert op.read_errors() == BAD_PAGE | POSITION
+    where = appended(table, lengths, counts, page)
+    dead = [w[0] for w in where if w[1] < 0 or w[3] >= 1029]
+    assert len(dead) == page + 1
+    where = [w for w in where if w[0] not in dead]
+    i, pg, off, pos = (torch.tensor(x, dtype=torch.int64) for x in zip(*where))
+    if with_q:
+        close(out[i], *exact(q[i], qw, pos, rope, False))
+        assert not out[tokens:].any() and not out[dead].any()
+    close(kc[pg, off], *exact(k[i], kw, pos, rope, False))
+    assert torch.equal(vc[pg, off], v[i])
+    kc[pg, off], vc[pg, off] = before[0][pg, off], before[1][pg, off]
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
 
 
 def test_append_without_rotation_copies_bits():
