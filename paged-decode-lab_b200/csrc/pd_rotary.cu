@@ -52,7 +52,8 @@ constexpr int kRows = 4, kMaxThreads = 512;
 // The streaming kernel: consumer warps beside one producer warp, CTAs per SM and
 // the shared memory of each one's stages.
 constexpr int kConsumers = 8, kStreamCtas = 3, kStreamThreads = 32 * (kConsumers + 1);
-constexpr int kMaxStages = 8, kMinStages = 3, kRingBytes = 70 * 1024;
+constexpr int kMaxStages = 8, kMinStages = 3;
+constexpr int kRingBytes[kStreamCtas + 1] = {0, 208 * 1024, 104 * 1024, 70 * 1024};   // by CTAs per SM
 constexpr uint32_t kErrBadPage = PD_DEVERR_BAD_PAGE, kErrLength = PD_DEVERR_LENGTH, kErrPosition = PD_DEVERR_POSITION;
 
 // One thread's part of a row: two pieces of 8 bytes, each moved whole when
@@ -272,7 +273,7 @@ struct Lane {
     }
 };
 
-// Direct kernel: any strides and alignment, few tokens.  One CTA per token; its
+// Direct kernel: any strides, alignment and size.  One CTA per token; its
 // row slots take rows slot, slot + slots, .. of [queries][keys][values], kRows of
 // them in flight before the token's place is looked up.
 template <typename Elt, int D, bool VECTOR, bool APPEND, bool INTERLEAVED>
@@ -362,8 +363,7 @@ struct StreamShape {
     size_t smem;
 };
 
-// Streaming kernel: many tokens whose rows lie one after another (16-byte
-// aligned).  A persistent CTA takes every gridDim-th token through a ring of
+// Streaming kernel: tokens whose rows lie one after another (16-byte aligned).  A persistent CTA takes every gridDim-th token through a ring of
 // stages: the producer warp brings a token's queries, keys, values and its
 // row of the rotation table by bulk copies, the consumer warps norm and rotate
 // the rows where they are, and the producer sends the whole token on by bulk
@@ -487,6 +487,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) rotary_stream_ker
             // rows of one kind: PER_WARP for each warp at a time, beginning with warp `first`
             const auto work = [&](Elt *rows, int heads, int first, bool norms, const f32x2 (&lo)[W], const f32x2 (&hi)[W]) {
                 if (!norms && !a.table && live) return;
+#pragma unroll 2
                 for (int base = first * PER_WARP; base < heads; base += kConsumers * PER_WARP) {
                     const int row = base + lane / LANES;
                     Elt *x = rows + row * D;
@@ -536,7 +537,7 @@ std::set<std::pair<int, const void *>> g_stream_done;
 cudaError_t allow_stream_smem(int device, const void *kernel) {
     std::lock_guard<std::mutex> lock(g_stream_mutex);
     if (g_stream_done.count({device, kernel})) return cudaSuccess;
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes + 4096);
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes[1] + 1024);
     if (err == cudaSuccess) g_stream_done.insert({device, kernel});
     return err;
 }
@@ -552,21 +553,26 @@ cudaError_t launch_rotary(const RotaryArgs &a, Alignment align, int device, cuda
     int sms = 148;
     cudaError_t err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (err != cudaSuccess) return err;
-    // Streaming pays when each of its CTAs has several tokens to overlap.
+    // Streaming wherever the rows allow it and three tokens fit an SM, in as many CTAs as then have
+    // three stages.  Against the direct kernel, us at 16 / 148 / 600 / 2000 tokens: rotating 32:8 FP16
+    // heads of 128 3.1 / 3.2 / 5.7 / 10.9 against 4.3 / 4.5 / 7.1 / 14.0, appending 64:8 of them
+    // 4.2 / 4.4 / 8.1 / 16.0 against 5.2 / 5.3 / 11.0 / 28.3.
     StreamShape sh{};
     const int row = D * int(sizeof(Elt));
-    const int64_t token_bytes = int64_t(a.q.heads + a.k.heads + a.v.heads) * row + a.rotary * 4;
-    if (align.rows && a.tokens >= int64_t(kStreamCtas) * sms * kMinStages && token_bytes * kMinStages <= kRingBytes) {
+    const int64_t token_bytes = (int64_t(a.q.heads + a.k.heads + a.v.heads) * row + a.rotary * 4 + 127) / 128 * 128;
+    int ctas = kStreamCtas;
+    while (ctas > 0 && token_bytes * kMinStages > kRingBytes[ctas]) --ctas;
+    if (align.rows && ctas > 0) {
         sh.q_bytes = a.q.heads * row;
         sh.k_bytes = a.k.heads * row;
         sh.v_bytes = a.v.heads * row;
-        sh.stage_bytes = int((token_bytes + 127) / 128 * 128);
-        sh.stages = std::min(kMaxStages, kRingBytes / sh.stage_bytes);
+        sh.stage_bytes = int(token_bytes);
+        sh.stages = std::min(kMaxStages, kRingBytes[ctas] / sh.stage_bytes);
         sh.smem = size_t(sh.stages) * sh.stage_bytes + kMaxStages * (8 + 8 + 8 + 4);
         const auto kernel = rotary_stream_kernel<Elt, D, APPEND, INTERLEAVED>;
         err = allow_stream_smem(device, reinterpret_cast<const void *>(kernel));
         if (err != cudaSuccess) return err;
-        return launch_dependent(kernel, std::min<int64_t>(a.tokens, int64_t(kStreamCtas) * sms), kStreamThreads, sh.smem,
+        return launch_dependent(kernel, std::min<int64_t>(a.tokens, int64_t(ctas) * sms), kStreamThreads, sh.smem,
                                 stream, a, sh);
     }
     // row slots: a thread's kRows rows cover the token, in whole warps

@@ -130,6 +130,12 @@ def load():
     return _lib
 
 
+def stream_of(device_index: int) -> int:
+    """The current CUDA stream of a device, as the library takes it."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def check(status: int, what: str = "") -> None:
     """Map a pd_status to the reference's Python exception types."""
     if status == PD_OK:

@@ -113,6 +113,7 @@ class SharedPrefixPlan:
         self._q_shape = (layout.batch, layout.query_heads, layout.head_dim)
         self._k_shape = (layout.physical_pages, layout.page_size, layout.kv_heads, layout.head_dim)
         self._out = torch.empty(self._q_shape, dtype=dtype, device=self.device)
+        self._index = self.device.index
 
     def __del__(self):
         handle = getattr(self, "_handle", None)
@@ -126,7 +127,7 @@ class SharedPrefixPlan:
         return int(self._buffer.numel())
 
     def _check(self, q, k, v, out):
-        index, dtype = self.device.index, self.dtype
+        index, dtype = self._index, self.dtype
         if q.shape != self._q_shape or k.shape != self._k_shape or v.shape != self._k_shape:
             raise ValueError("input shape does not match plan")
         if q.dtype != dtype or k.dtype != dtype or v.dtype != dtype:
@@ -144,10 +145,9 @@ class SharedPrefixPlan:
 
     def run(self, q, k, v, out=None):
         """Decode one step; returns the plan's borrowed output, or writes into ``out`` and returns it."""
-        import torch
         out = self._check(q, k, v, out)
         status = self._lib.pd_prefix_decode(self._handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), self._code,
-                                            out.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+                                            out.data_ptr(), _native.stream_of(self._index))
         if status:
             _native.check(status, "decode")
         return out
@@ -159,16 +159,15 @@ class SharedPrefixPlan:
         sequence whose live length ends inside its prefix (0: not in use)
         attends to its live tokens only.
         """
-        import torch
         if self.max_lengths is None:
             raise ValueError("run_dynamic needs a plan built with max_lengths")
         out = self._check(q, k, v, out)
-        index, batch = self.device.index, self.layout.batch
+        index, batch = self._index, self.layout.batch
         table_at = _int32(table, (batch, self._width), "table", index)
         lengths_at = _int32(lengths, (batch,), "lengths", index)
         status = self._lib.pd_prefix_decode_dynamic(
             self._handle, q.data_ptr(), k.data_ptr(), v.data_ptr(), self._code, table_at, lengths_at, out.data_ptr(),
-            torch.cuda.current_stream(self.device).cuda_stream)
+            _native.stream_of(index))
         if status:
             _native.check(status, "decode")
         return out

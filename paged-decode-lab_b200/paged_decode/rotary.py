@@ -46,35 +46,35 @@ def _cuda_device(device):
     return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
 
 
-def _fill(rows, x, out, name, heads, head_dim, dtype, index, tokens):
-    """Check x (and out) [tokens, heads, head_dim] and describe them to the library."""
-    if tuple(x.shape) != (tokens, heads, head_dim):
-        raise ValueError(f"{name} must have shape [{tokens}, {heads}, {head_dim}]")
+def _refuse_rows(x, name, shape, dtype, index):
+    """Raise for the first thing that is wrong with heads x."""
+    if tuple(x.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}")
     if x.dtype != dtype:
         raise TypeError("q/k/v, their outputs and the caches must share float16 or float32 dtype")
-    strides = x.stride()
-    if x.get_device() != index or strides[2] != 1:
+    if x.get_device() != index or x.stride(2) != 1:
         raise ValueError(f"{name} must be on the device, its last dim contiguous")
-    if x.requires_grad:
-        raise ValueError("inference only: detach tensors requiring gradients")
-    rows.data, rows.token_stride, rows.head_stride, rows.heads = x.data_ptr(), strides[0], strides[1], heads
+    raise ValueError("inference only: detach tensors requiring gradients")
+
+
+def _fill(rows, x, out, name, shape, dtype, index):
+    """Check x (and out) [tokens, heads, head_dim] and describe them to the library."""
+    strides = x.stride()
+    if x.shape != shape or x.dtype != dtype or x.get_device() != index or strides[2] != 1 or x.requires_grad:
+        _refuse_rows(x, name, shape, dtype, index)
+    rows.data, rows.token_stride, rows.head_stride, rows.heads = x.data_ptr(), strides[0], strides[1], shape[1]
     if out is not None:
         if out is not x:
-            if out.shape != x.shape:
-                raise ValueError(f"{name}_out must have {name}'s shape")
-            if out.dtype != dtype:
-                raise TypeError("q/k/v, their outputs and the caches must share float16 or float32 dtype")
             strides = out.stride()
-            if out.get_device() != index or strides[2] != 1:
-                raise ValueError(f"{name}_out must be on the device, its last dim contiguous")
-            if out.requires_grad:
-                raise ValueError("inference only: detach tensors requiring gradients")
+            if out.shape != shape or out.dtype != dtype or out.get_device() != index or strides[2] != 1 or \
+                    out.requires_grad:
+                _refuse_rows(out, f"{name}_out", shape, dtype, index)
         rows.out, rows.out_token_stride, rows.out_head_stride = out.data_ptr(), strides[0], strides[1]
 
 
 def _int32(t, shape, name, index):
     import torch
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != shape or \
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != shape or \
             t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 CUDA tensor of shape {list(shape)} on the device")
     return t.data_ptr()
@@ -121,6 +121,7 @@ class HeadRotation:
         self.table, (self.q_weight, self.k_weight) = table, weights
         self._lib = _native.load()
         self._error = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._error_at, self._index = self._error.data_ptr(), self.device.index
         self._spec = _native.Rotation(head_dim, self.rotary_dim, int(self.interleaved), self.eps, self.max_positions,
                                       *(None if t is None else t.data_ptr() for t in (table, *weights)))
         self._rows = [_native.Heads(), _native.Heads()]
@@ -141,7 +142,7 @@ class HeadRotation:
             raise ValueError("q or k is needed")
         if first.ndim != 3:
             raise ValueError("heads must have shape [tokens, heads, head_dim]")
-        dtype, index, tokens = first.dtype, self.device.index, first.shape[0]
+        dtype, index, tokens = first.dtype, self._index, first.shape[0]
         code = _dtype_code(dtype, "q/k")
         outs, refs = [], []
         for name, x, out, rows, ref in (("q", q, q_out, self._rows[0], self._refs[1]),
@@ -155,12 +156,12 @@ class HeadRotation:
                     raise ValueError("heads must have shape [tokens, heads, head_dim]")
                 if out is None:
                     out = torch.empty(x.shape, dtype=dtype, device=self.device)
-                _fill(rows, x, out, name, x.shape[1], self.head_dim, dtype, index, tokens)
+                _fill(rows, x, out, name, (tokens, x.shape[1], self.head_dim), dtype, index)
             outs.append(out)
             refs.append(ref)
         status = self._lib.pd_rotate_heads(
             self._refs[0], refs[0], refs[1], tokens, _int32(positions, (tokens,), "positions", index), code,
-            self._error.data_ptr(), index, torch.cuda.current_stream(self.device).cuda_stream)
+            self._error_at, index, _native.stream_of(index))
         if status:
             _native.check(status, "rotate")
         return tuple(outs)
@@ -194,6 +195,7 @@ class CacheAppend:
         self.layout, self.rotation = layout, rotation
         self._lib = _native.load()
         self._error = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._error_at, self._index = self._error.data_ptr(), self.device.index
         self._layout = _native.Layout(layout.batch, layout.query_heads, layout.kv_heads, layout.head_dim,
                                       layout.page_size, layout.physical_pages)
         self._cache_shape = (layout.physical_pages, layout.page_size, layout.kv_heads, layout.head_dim)
@@ -216,7 +218,7 @@ class CacheAppend:
         (``read_errors``).  All device inputs are read when the kernel runs.
         """
         import torch
-        layout, index = self.layout, self.device.index
+        layout, index = self.layout, self._index
         if k.ndim != 3:
             raise ValueError("heads must have shape [tokens, heads, head_dim]")
         dtype, tokens, dim = k.dtype, k.shape[0], layout.head_dim
@@ -225,21 +227,17 @@ class CacheAppend:
         if q is not None:
             if q_out is None:
                 q_out = torch.empty((tokens, layout.query_heads, dim), dtype=dtype, device=self.device)
-            _fill(self._rows[0], q, q_out, "q", layout.query_heads, dim, dtype, index, tokens)
+            _fill(self._rows[0], q, q_out, "q", (tokens, layout.query_heads, dim), dtype, index)
             q_ref = self._refs[2]
         elif q_out is not None:
             raise ValueError("q_out without q")
-        _fill(self._rows[1], k, None, "k", layout.kv_heads, dim, dtype, index, tokens)
-        _fill(self._rows[2], v, None, "v", layout.kv_heads, dim, dtype, index, tokens)
+        shape = (tokens, layout.kv_heads, dim)
+        _fill(self._rows[1], k, None, "k", shape, dtype, index)
+        _fill(self._rows[2], v, None, "v", shape, dtype, index)
         for cache in (k_cache, v_cache):
-            if tuple(cache.shape) != self._cache_shape:
-                raise ValueError("cache shape does not match the layout")
-            if cache.dtype != dtype:
-                raise TypeError("q/k/v, their outputs and the caches must share float16 or float32 dtype")
-            if cache.get_device() != index or not cache.is_contiguous():
-                raise ValueError("caches must be contiguous on the device")
-            if cache.requires_grad:
-                raise ValueError("inference only: detach tensors requiring gradients")
+            if cache.shape != self._cache_shape or cache.dtype != dtype or cache.get_device() != index or \
+                    not cache.is_contiguous() or cache.requires_grad:
+                self._refuse_cache(cache, dtype, index)
         if indptr is None:
             if tokens != layout.batch:
                 raise ValueError("without indptr there is one token per sequence")
@@ -252,10 +250,19 @@ class CacheAppend:
         status = self._lib.pd_cache_append(
             self._refs[0], self._refs[1], q_ref, self._refs[3], self._refs[4], tokens, k_cache.data_ptr(),
             v_cache.data_ptr(), code, _int32(table, (layout.batch, width), "table", index), width,
-            _int32(lengths, (layout.batch,), "lengths", index), indptr_at, self._error.data_ptr(), index,
-            torch.cuda.current_stream(self.device).cuda_stream)
+            _int32(lengths, (layout.batch,), "lengths", index), indptr_at, self._error_at, index,
+            _native.stream_of(index))
         if status:
             _native.check(status, "append")
         return q_out
+
+    def _refuse_cache(self, cache, dtype, index):
+        if tuple(cache.shape) != self._cache_shape:
+            raise ValueError("cache shape does not match the layout")
+        if cache.dtype != dtype:
+            raise TypeError("q/k/v, their outputs and the caches must share float16 or float32 dtype")
+        if cache.get_device() != index or not cache.is_contiguous():
+            raise ValueError("caches must be contiguous on the device")
+        raise ValueError("inference only: detach tensors requiring gradients")
 
     read_errors = HeadRotation.read_errors
