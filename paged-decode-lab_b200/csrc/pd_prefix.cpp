@@ -123,12 +123,12 @@ struct SimtShape {
     static constexpr int64_t rows = 16, step_tokens = 32, ctas_per_sm = 4;
 };
 
-// FP16 (tcgen05): tiles of 128 rows, 128-token steps, one CTA per SM with two
+// FP16 (tcgen05): tiles of 128 rows, 64-token steps, one CTA per SM with two
 // streams (see pd_prefix_mma.cuh).
 struct MmaShape {
-    static constexpr int64_t rows = 128, step_tokens = 128;
+    static constexpr int64_t rows = 128, step_tokens = 64;
     // start and end of a CTA (launch, first loads, the partials' store), in steps
-    static constexpr int64_t overhead_steps = 3;
+    static constexpr int64_t overhead_steps = 8;
 };
 
 }  // namespace
@@ -236,6 +236,14 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
         pages.insert(pages.end(), row, row + g.pages);
     }
     p.slots = int32_t(slots);
+    // Merge: at most four pieces (one batch of loads) per thread set, while the
+    // sets' threads still fit the device at once (2048 per SM).
+    int32_t most_pieces = 1;
+    for (size_t t = 1; t < p.tiles.size(); t += 2) most_pieces = std::max(most_pieces, p.tiles[t]);
+    p.merge_ways = 1;
+    while (p.merge_ways < 8 && p.merge_ways * 4 < most_pieces &&
+           int64_t(L.batch) * L.query_heads * (D / 8) * p.merge_ways * 2 <= int64_t(sm_count) * 2048)
+        p.merge_ways *= 2;
 
     PrefixImage &im = p.image;
     size_t off = 0;

@@ -118,10 +118,10 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
 #pragma unroll
     for (int x = 4; x > 0; x >>= 1) l += __shfl_xor_sync(kFullMask, l, x);
     if (on) {
-        float *po = a.part_o + (int64_t(i1.w) * R + r) * D;
+        float *po = a.part_o + int64_t(i1.w) * R * D + r * 8 + c % 2 * 4;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
-            *reinterpret_cast<float4 *>(po + 32 * d + 4 * c) =
+            *reinterpret_cast<float4 *>(po + (4 * d + c / 2) * (R * 8)) =
                 make_float4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
         if (c == 0) a.part_ml[int64_t(i1.w) * R + r] = make_float2(m, l);
     }
@@ -129,105 +129,147 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// (m, l) of one row over the first `limit` tokens of its prefix, o in `o`: for a
-// dynamic launch's sequence that ends inside its prefix, whose row in the
-// group's matrix covers the whole prefix.  One warp, a token at a time: such
-// lengths are rare, and most of them 0.
+// (m, l) of one row over the first `limit` tokens of its prefix, and in `o`
+// eight dims of it: for a dynamic launch's sequence that ends inside its prefix,
+// whose row in the group's matrix covers the whole prefix.  D / 8 neighbouring
+// lanes, a token at a time: such lengths are rare, and most of them 0.
 template <typename Elt, int D>
 __device__ __noinline__ float2 prefix_row(const PrefixArgs &a, int64_t row, int kv_head, const int32_t *pages,
-                                          int limit, int lane, float (&o)[D / 32]) {
-    constexpr int N = D / 32;
-    float q[N], m = -INFINITY, l = 0.f;
+                                          int limit, int lane, float (&o)[8]) {
+    constexpr int LANES = D / 8;
+    const unsigned mates = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+    float q[8], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        q[i] = float(static_cast<const Elt *>(a.q)[row * D + lane * N + i]) * a.scale_log2;
+    for (int i = 0; i < 8; ++i) {
+        q[i] = float(static_cast<const Elt *>(a.q)[row * D + lane * 8 + i]) * a.scale_log2;
         o[i] = 0.f;
     }
     for (int t = 0; t < limit; ++t) {
         const int64_t at = ((int64_t(pages[t / a.page_size]) * a.page_size + t % a.page_size) * a.Hkv + kv_head) * D +
-                           lane * N;
+                           lane * 8;
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(q[i], float(static_cast<const Elt *>(a.k)[at + i]), s);
+        for (int i = 0; i < 8; ++i) s = fmaf(q[i], float(static_cast<const Elt *>(a.k)[at + i]), s);
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(kFullMask, s, x);
+        for (int x = LANES / 2; x > 0; x >>= 1) s += __shfl_xor_sync(mates, s, x);
         const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
         const float shrink = exp2f(m - base), p = exp2f(s - base);
         l = fmaf(l, shrink, p);
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(o[i], shrink, p * float(static_cast<const Elt *>(a.v)[at + i]));
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], shrink, p * float(static_cast<const Elt *>(a.v)[at + i]));
         m = top;
     }
     return make_float2(m, l);
 }
 
-// One warp per output row: the suffix's normalised row and the prefix pieces,
-// in piece order, each scaled to the common maximum.
+// Eight FP32 values to eight elements, one rounding each.
+__device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
+    *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4 *>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__half *dst, const float (&x)[8]) {
+    *reinterpret_cast<uint4 *>(dst) =
+        make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+}
+
+// A part of a row: softmax statistics and this thread's eight dims, o not normalised.
+struct RowPart {
+    float m = -INFINITY, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // Take in (m2, l2, x).  Parts without a token have l2 = 0; a NaN denominator stays one.
+    __device__ __forceinline__ void absorb(float m2, float l2, const float (&x)[8]) {
+        if (l2 == 0.f) return;
+        const float top = fmaxf(m, m2);
+        const float f = m == top ? 1.f : exp2f(m - top), g = exp2f(m2 - top);
+        l = fmaf(l, f, l2 * g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], f, x[i] * g);
+        m = top;
+    }
+};
+
+// Each output row from the suffix's normalised row and the prefix pieces: D / 8
+// threads per row, eight dims each, and `ways` such sets per row that take every
+// ways-th piece (several where rows are few and pieces many); the sets' parts are
+// merged in order.  What a row needs to know is looked up before the
+// prefix kernel is waited for; pieces are loaded four at a time.
+constexpr int kMergeThreads = 256;
 template <typename Elt, int D>
-__global__ void __launch_bounds__(256) prefix_merge_kernel(const PrefixArgs a) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t out_row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (out_row >= int64_t(a.B) * a.Hq) return;
-    const int lane = threadIdx.x & 31;
-    constexpr int N = D / 32;                                   // dims per lane
-    const int b = int(out_row / a.Hq), head = int(out_row % a.Hq);
-    const int4 sq = a.seqs[2 * b];
-    int64_t slot = 0;
-    int r = 0, pieces = 0;
-    float2 own = make_float2(-INFINITY, 0.f);                   // a prefix part computed here
-    float oo[N];
+__global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const PrefixArgs a, int ways) {
+    constexpr int LANES = D / 8, BATCH = 4;
+    __shared__ RowPart parts[kMergeThreads];
+    const int per_cta = kMergeThreads / LANES / ways;
+    const int set = threadIdx.x / LANES, way = set % ways, lane = threadIdx.x % LANES;
+    const int64_t out_row = int64_t(blockIdx.x) * per_cta + set / ways;
+    const bool on = out_row < int64_t(a.B) * a.Hq;
+    const int b = on ? int(out_row / a.Hq) : 0, head = int(out_row % a.Hq);
+    const int4 sq = on ? __ldg(a.seqs + 2 * b) : make_int4(-1, 0, 0, 0);
+    int pieces = 0, prefix_pages = 0;
+    const float2 *ml = a.part_ml;
+    const float *po = a.part_o;
     if (sq.x >= 0) {
         const int row = sq.x * a.group + head % a.group;
-        const int2 tile = a.tiles[sq.y + int64_t(head / a.group) * sq.z + row / a.tile_rows];
-        slot = tile.x;
+        const int2 tile = __ldg(a.tiles + sq.y + int64_t(head / a.group) * sq.z + row / a.tile_rows);
+        prefix_pages = __ldg(a.seqs + 2 * b + 1).x;
         pieces = tile.y;
-        r = row % a.tile_rows;
-        if constexpr (sizeof(Elt) == 2) {
-            const int limit = __ldcg(a.lengths + b);
-            if (limit < a.seqs[2 * b + 1].x * a.page_size) {
-                pieces = 0;
-                own = prefix_row<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, limit, lane, oo);
-            }
+        ml += int64_t(tile.x) * a.tile_rows + row % a.tile_rows;
+        po += int64_t(tile.x) * a.tile_rows * D + lane * (a.tile_rows * 8) + row % a.tile_rows * 8;
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    RowPart part;
+    // a dynamic launch's sequence that ends inside its prefix
+    const bool inside = sizeof(Elt) == 2 && prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size;
+    if (inside) pieces = 0;
+    if (way == 0 && on) {
+        float2 suffix = make_float2(-INFINITY, 0.f);
+        if (a.rows) suffix = __ldcg(reinterpret_cast<const float2 *>(a.stats) + out_row);
+        if (suffix.y != 0.f) {
+            const float4 *x = reinterpret_cast<const float4 *>(a.rows + out_row * D + lane * 8);
+            const float4 u = __ldcg(x), v = __ldcg(x + 1);
+            const float o[8] = {u.x * suffix.y, u.y * suffix.y, u.z * suffix.y, u.w * suffix.y,
+                                v.x * suffix.y, v.y * suffix.y, v.z * suffix.y, v.w * suffix.y};
+            part.absorb(suffix.x, suffix.y, o);
+        }
+        if (inside) {
+            float o[8];
+            const float2 own = prefix_row<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, __ldcg(a.lengths + b), lane, o);
+            part.absorb(own.x, own.y, o);
         }
     }
-    float2 suffix = make_float2(-INFINITY, 0.f);
-    if (a.rows) suffix = reinterpret_cast<const float2 *>(a.stats)[out_row];
-    // parts with no token have l = 0; a NaN denominator stays one
-    float top = suffix.y != 0.f ? suffix.x : -INFINITY;
-    if (own.y != 0.f) top = fmaxf(top, own.x);
-    for (int p = 0; p < pieces; ++p) {
-        const float2 ml = a.part_ml[(slot + p) * a.tile_rows + r];
-        if (ml.y != 0.f) top = fmaxf(top, ml.x);
+    const int64_t ml_step = a.tile_rows, o_step = int64_t(a.tile_rows) * D;
+    for (int p0 = way; p0 < pieces; p0 += ways * BATCH) {
+        float2 st[BATCH];
+        float4 u[BATCH], v[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const int p = p0 + j * ways;
+            st[j] = make_float2(-INFINITY, 0.f);
+            if (p < pieces) {
+                st[j] = __ldcg(ml + p * ml_step);
+                const float4 *x = reinterpret_cast<const float4 *>(po + p * o_step);
+                u[j] = __ldcg(x);
+                v[j] = __ldcg(x + 1);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const float o[8] = {u[j].x, u[j].y, u[j].z, u[j].w, v[j].x, v[j].y, v[j].z, v[j].w};
+            part.absorb(st[j].x, st[j].y, o);
+        }
     }
-    float den = 0.f, o[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.f;
-    if (suffix.y != 0.f) {
-        den = suffix.y * exp2f(suffix.x - top);
-        const float *x = a.rows + out_row * D + lane * N;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = den * x[i];
+    if (ways > 1) {
+        parts[threadIdx.x] = part;
+        __syncthreads();
+        if (way != 0) return;
+        for (int w = 1; w < ways; ++w) {
+            const RowPart other = parts[threadIdx.x + w * LANES];
+            part.absorb(other.m, other.l, other.o);
+        }
     }
-    if (own.y != 0.f) {
-        const float w = exp2f(own.x - top);
-        den = fmaf(w, own.y, den);
+    if (!on) return;
+    const float inv = part.l != 0.f ? 1.f / part.l : 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(w, oo[i], o[i]);
-    }
-    for (int p = 0; p < pieces; ++p) {
-        const int64_t at = (slot + p) * a.tile_rows + r;
-        const float2 ml = a.part_ml[at];
-        if (ml.y == 0.f) continue;
-        const float w = exp2f(ml.x - top);
-        den = fmaf(w, ml.y, den);
-        const float *x = a.part_o + at * D + lane * N;
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(w, x[i], o[i]);
-    }
-    const float inv = den != 0.f ? 1.f / den : 0.f;
-    Elt *dst = static_cast<Elt *>(a.out) + out_row * D + lane * N;
-#pragma unroll
-    for (int i = 0; i < N; ++i) dst[i] = Elt(o[i] * inv);
+    for (int i = 0; i < 8; ++i) part.o[i] *= inv;
+    store8(static_cast<Elt *>(a.out) + out_row * D + lane * 8, part.o);
 }
 
 template <typename... Params, typename... Args>
@@ -273,9 +315,11 @@ cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CU
         err = launch_dependent(prefix_simt_kernel<float, D>, items, kSimtThreads, 0, stream, a);
     }
     if (err != cudaSuccess) return err;
-    const int64_t grid = (int64_t(a.B) * a.Hq + 7) / 8;
-    return p.dtype == PD_FLOAT16 ? launch_dependent(prefix_merge_kernel<__half, D>, grid, 256, 0, stream, a)
-                                 : launch_dependent(prefix_merge_kernel<float, D>, grid, 256, 0, stream, a);
+    const int64_t rows = int64_t(a.B) * a.Hq, per_cta = kMergeThreads / (D / 8) / p.merge_ways;
+    const int64_t grid = (rows + per_cta - 1) / per_cta;
+    return p.dtype == PD_FLOAT16
+               ? launch_dependent(prefix_merge_kernel<__half, D>, grid, kMergeThreads, 0, stream, a, p.merge_ways)
+               : launch_dependent(prefix_merge_kernel<float, D>, grid, kMergeThreads, 0, stream, a, p.merge_ways);
 }
 
 pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const void *v, pd_dtype dtype,

@@ -23,7 +23,7 @@ struct PrefixArgs {
     const int32_t *lengths;     // [B]
     const float *rows;          // the suffix decode: FP32 [B, Hq, D] and (m, l) [B, Hq, 2]; NULL: no suffix
     const float *stats;
-    float *part_o;              // [slots][tile rows][D]
+    float *part_o;              // [slots][D / 8][tile rows][8]
     float2 *part_ml;            // [slots][tile rows]
     void *out;                  // [B, Hq, D]
     uint32_t *error;

@@ -1,7 +1,7 @@
 // pd_prefix_mma.cuh — the FP16 shared-prefix kernel on the 5th-generation tensor cores.
 //
 // One CTA per work item.  An item has up to two streams, each one tile of 128
-// query rows against a run of prefix pages, 128 tokens a step:
+// query rows against a run of prefix pages, 64 tokens a step:
 //   * paired: two row tiles of one (group, KV head) over the same pages; each
 //     K and V step is loaded once and used by both;
 //   * split: one row tile whose pages are cut in two runs; each stream loads
@@ -14,10 +14,13 @@
 //     its A operand;
 //   * warp 8, two lanes: TMA loads of K and V steps into one ring (one lane its
 //     even slots, one its odd slots), one box per page;
-//   * warp 9, one thread: the MMAs.  S = Q K^T (M 128, N 128), O += P V (M 128,
-//     N = head dim).  While one stream's softmax works, the other's products run.
-// The scores of step i + 1 overwrite the weights of step i, so they are issued
-// once the PV product of step i has completed.
+//   * warp 9, one elected lane: the MMAs.  S = Q K^T (M 128, N 64), O += P V (M 128,
+//     N = head dim).
+// Each stream has two score blocks, so that a softmax finds its next scores
+// ready: those of step i + 2 are issued once the PV product of step i, whose
+// weights lie in the same block, has completed.  (Steps of 128 tokens leave
+// tensor memory for one block per stream: every step then waited for PV, QK and
+// softmax one after another, 2.7 us a pair of 128-token steps at head_dim 128.)
 //
 // Softmax in base 2 with a reference m that moves only when a score passes it
 // by more than 2^15 (then O is rescaled in tensor memory): a fresh reference is
@@ -28,7 +31,7 @@
 // so no scores need masks; a last step of fewer pages takes fewer columns.
 //
 // Every wait is bounded; on a timeout the CTA records PD_DEVERR_TIMEOUT,
-// unwinds, waits for its own MMAs and frees its tensor memory.
+// unwinds, waits for its own MMAs and copies and frees its tensor memory.
 #pragma once
 
 #include "paged_decode.h"
@@ -40,21 +43,23 @@ namespace pd {
 
 template <int D, int T>
 struct PrefixShape {
-    static constexpr int M = 128, NS = 128;             // rows of a tile, tokens of a step
+    static constexpr int M = 128, NS = 64;              // rows of a tile, tokens of a step
     static constexpr int NP = NS / T;                   // pages of a step
     static constexpr int NBOX = D * 2 / 128;            // 128-byte boxes per row
     static constexpr int PAGE_BYTES = T * D * 2;        // K (or V) rows of one page and head
     static constexpr int STEP_BYTES = NP * PAGE_BYTES;
     static constexpr int Q_BOX = M * 128;
     static constexpr int Q_BYTES = NBOX * Q_BOX;
-    static constexpr int SLOTS = D == 128 ? 5 : 8;      // ring slots of one K or V step
+    static constexpr int SLOTS = D == 128 ? 10 : 16;    // ring slots of one K or V step; even: a lane's slots stay its own
     static constexpr int SOFTMAX_WARPS = 8, W_LOAD = 8, W_MMA = 9;
     static constexpr int THREADS = 320;
-    static constexpr int S_COL = 0, O_COL = 2 * NS;     // tensor memory: [S0 | P0][S1 | P1][O0][O1]
+    // tensor memory: score blocks (weights in their first half) [stream][2], outputs [stream]
+    static constexpr int S_COL = 0, O_COL = 4 * NS;
     static constexpr int TMEM_COLS = 512;
-    static constexpr int NBARS = 2 * SLOTS + 2 * 4 + 1;
+    static constexpr int NBARS = 2 * SLOTS + 2 + 4 + 4 + 2 + 1;
     static constexpr size_t SMEM = 1024 + 2 * size_t(Q_BYTES) + size_t(SLOTS) * STEP_BYTES + NBARS * 8 + 16;
     static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory budget");
+    static_assert(SLOTS % 2 == 0, "a slot belongs to one lane");
     static_assert(SMEM <= 232448 && SMEM > 116 * 1024, "one CTA per SM: tensor memory is never contended");
 };
 
@@ -96,22 +101,26 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixArgs &a, int i) {
     return it;
 }
 
-// The order in which the MMA thread uses the ring: the first K of each stream,
-// then per step and stream V and the next K; paired streams share stream 0's.
-// use(position, stream, is_v, step) is called for each.
+// The order in which the MMA thread first uses the ring: use(position, stream,
+// is_v, step) for each.  Paired streams share stream 0's steps.
 template <typename Use>
 __device__ __forceinline__ void ring_order(int n0, int n1, bool paired, Use use) {
-    const int streams = paired ? 1 : 2;
+    if (paired) n1 = 0;
     int pos = 0;
-    for (int t = 0; t < streams; ++t)
-        if ((t ? n1 : n0) > 0 && !use(pos++, t, false, 0)) return;
-    for (int i = 0; i < n0; ++i)
-        for (int t = 0; t < streams; ++t) {
-            const int n = t ? n1 : n0;
-            if (i < n && !use(pos++, t, true, i)) return;
-            if (i + 1 < n && !use(pos++, t, false, i + 1)) return;
-        }
+    for (int i = 0; i < 2; ++i) {
+        if (i < n0 && !use(pos++, 0, false, i)) return;
+        if (i < n1 && !use(pos++, 1, false, i)) return;
+    }
+    for (int i = 0; i < n0; ++i) {
+        if (!use(pos++, 0, true, i)) return;
+        if (i > 0 && i + 1 < n1 && !use(pos++, 1, false, i + 1)) return;
+        if (i < n1 && !use(pos++, 1, true, i)) return;
+        if (i + 2 < n0 && !use(pos++, 0, false, i + 2)) return;
+    }
 }
+// Paired: the positions of K step j and V step i of n.
+__device__ __forceinline__ int paired_k(int j) { return j < 2 ? j : 2 * j - 1; }
+__device__ __forceinline__ int paired_v(int i, int n) { return min(n, 2) + i + min(i, max(n - 2, 0)); }
 
 template <int D, int T>
 __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
@@ -126,14 +135,14 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + size_t(SLOTS) * S::STEP_BYTES);
     uint64_t *empty = full + SLOTS;
     uint64_t *q_full = empty + SLOTS;       // [2] query rows written (4 warps)
-    uint64_t *s_full = q_full + 2;          // [2] scores done
-    uint64_t *p_full = s_full + 2;          // [2] weights written (4 warps)
-    uint64_t *o_done = p_full + 2;          // [2] PV product done
+    uint64_t *s_full = q_full + 2;          // [stream][block] scores done
+    uint64_t *p_full = s_full + 4;          // [stream][block] weights written (4 warps)
+    uint64_t *o_done = p_full + 4;          // [stream] PV product done
     uint64_t *mma_done = o_done + 2;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(mma_done + 1);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1) + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = int(__reduce_max_sync(kFullMask, threadIdx.x >> 5)), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
             mbar_init(smem_u32(full + s), 1);
@@ -141,9 +150,11 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(smem_u32(q_full + t), 4);
-            mbar_init(smem_u32(s_full + t), 1);
-            mbar_init(smem_u32(p_full + t), 4);
             mbar_init(smem_u32(o_done + t), 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(smem_u32(s_full + 2 * t + b), 1);
+                mbar_init(smem_u32(p_full + 2 * t + b), 4);
+            }
         }
         mbar_init(smem_u32(mma_done), 1);
         *abort_flag = 0;
@@ -175,7 +186,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             tma_prefetch_descriptor(lane == 0 ? &tm_k : &tm_v);
             int last = -1;              // the last position this lane loaded
             ring_order(n0, n1, paired, [&](int pos, int t, bool is_v, int step) {
-                if ((pos % SLOTS & 1) != lane) return true;
+                if ((pos & 1) != lane) return true;
                 const int p0 = it.s(t).first + step * NP, n = min(NP, it.s(t).end - p0);
                 int ids[NP];
 #pragma unroll
@@ -203,86 +214,79 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 return true;
             });
             // no copy of this lane is in flight when the CTA ends, whatever became of its readers
-            for (int pos = last; pos >= 0 && pos > last - SLOTS; --pos)
-                if ((pos % SLOTS & 1) == lane && !mbar_wait(smem_u32(full + pos % SLOTS), (pos / SLOTS) & 1)) fail_wait();
+            for (int pos = last; pos >= 0 && pos > last - SLOTS; pos -= 2)
+                if (!mbar_wait(smem_u32(full + pos % SLOTS), (pos / SLOTS) & 1)) fail_wait();
         }
         __syncwarp();
     } else if (warp == S::W_MMA) {
-        // ------------------------------------------------------------ MMAs (one thread)
-        if (lane == 0) {
+        // ------------------------------------------------------------ MMAs (one elected lane)
+        {
+            // The warp stays converged and every operand is the same in all lanes (reductions over
+            // the warp give the compiler the proof), so that they live in uniform registers.
+            const auto uniform = [](int x) { return __reduce_max_sync(kFullMask, x); };
+            const int un0 = uniform(n0), un1 = uniform(n1);
+            const int pages0 = uniform(it.s0.end - it.s0.first), pages1 = uniform(it.s1.end - it.s1.first);
+            const bool upaired = uniform(it.paired) != 0;
+            const uint32_t utmem = __reduce_max_sync(kFullMask, tmem);
             constexpr uint32_t ID_S = tc::idesc_f16_f32(S::M, S::NS, false, false);   // Q, K: K-major
             constexpr uint32_t ID_O = tc::idesc_f16_f32(S::M, D, false, true);        // V: MN-major
+            const uint64_t q_desc = tc::smem_desc(smem_u32(qbuf), 16, 1024, tc::kSwizzle128);
+            const uint64_t k_desc = tc::smem_desc(smem_u32(ring), 16, S::NBOX * 1024, tc::kSwizzle128);
+            const uint64_t v_desc = tc::smem_desc(smem_u32(ring), T * 128, 1024, tc::kSwizzle128);
             bool ok = true;
-            int pos = 0;                // ring positions used
-            const auto take = [&]() {   // wait for the next position's data
-                ok = ok && mbar_wait(smem_u32(full + pos % SLOTS), (pos / SLOTS) & 1);
-                return smem_u32(ring + size_t(pos % SLOTS) * S::STEP_BYTES);
+            int pos = 0;                // split streams: ring positions used
+            const auto wait_for = [&](uint64_t *bar, int phase) {
+                ok = ok && __all_sync(kFullMask, mbar_wait(smem_u32(bar), uint32_t(phase & 1)));
+                return ok;
             };
-            const auto give = [&]() { tc::commit(smem_u32(empty + pos++ % SLOTS)); };
-            const auto scores = [&](int t, uint32_t kb) {
-                const uint32_t qa = smem_u32(qbuf + (paired ? t : 0) * S::Q_BYTES);
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint64_t ad =
-                        tc::smem_desc(qa + (kk >> 2) * S::Q_BOX + (kk & 3) * 32, 16, 1024, tc::kSwizzle128);
-                    const uint64_t bd =
-                        tc::smem_desc(kb + (kk >> 2) * 1024 + (kk & 3) * 32, 16, S::NBOX * 1024, tc::kSwizzle128);
-                    tc::mma_f16(tmem + S::S_COL + t * S::NS, ad, bd, ID_S, kk > 0 ? 1u : 0u);
-                }
-                tc::commit(smem_u32(s_full + t));
-            };
-            const auto products = [&](int t, uint32_t vb, int tokens, bool first) {
-#pragma unroll 1
-                for (int kk = 0; kk < tokens / 16; ++kk) {
-                    const uint32_t page = vb + kk * 16 / T * S::PAGE_BYTES;
-                    const uint64_t bd = tc::smem_desc(page + kk * 16 % T * 128, T * 128, 1024, tc::kSwizzle128);
-                    tc::mma_f16_ta(tmem + S::O_COL + t * D, tmem + S::S_COL + t * S::NS + kk * 8, bd, ID_O,
-                                   first && kk == 0 ? 0u : 1u);
-                }
-                tc::commit(smem_u32(o_done + t));
-            };
-            const int streams = n1 > 0 ? 2 : 1;
-            uint32_t kb = 0, vb = 0;
-            for (int t = 0; t < streams && ok; ++t) {
-                const bool own = t == 0 || !paired;     // this stream's first use of its ring position
-                if (own) kb = take();
-                if (t == 0 || paired) ok = ok && mbar_wait(smem_u32(q_full + t), 0);
-                if (!ok) break;
+            // S of step j of stream t into its block j % 2
+            const auto scores = [&](int t, int j) {
+                const int at = upaired ? paired_k(j) : pos++, slot = at % SLOTS;
+                if ((t == 0 || !upaired) && !wait_for(full + slot, at / SLOTS)) return;
                 tc::fence_after_sync();
-                scores(t, kb);
-                if (!paired || t == streams - 1) give();
+                const uint64_t ad = q_desc + (upaired && t ? S::Q_BYTES >> 4 : 0);
+                const uint64_t bd = k_desc + uint32_t(slot) * (S::STEP_BYTES >> 4);
+                const uint32_t d = utmem + S::S_COL + (2 * t + (j & 1)) * S::NS;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    tc::mma_f16_warp(d, ad + (((kk >> 2) * S::Q_BOX + (kk & 3) * 32) >> 4),
+                                bd + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), ID_S, kk > 0 ? 1u : 0u);
+                tc::commit_warp(smem_u32(s_full + 2 * t + (j & 1)));
+                if (!upaired || t == 1) tc::commit_warp(smem_u32(empty + slot));
+            };
+            // O += P V of step i of stream t
+            const auto products = [&](int t, int i, int n) {
+                const int at = upaired ? paired_v(i, n) : pos++, slot = at % SLOTS;
+                if ((t == 0 || !upaired) && !wait_for(full + slot, at / SLOTS)) return;
+                if (!wait_for(p_full + 2 * t + (i & 1), i >> 1)) return;
+                tc::fence_after_sync();
+                const uint64_t bd = v_desc + uint32_t(slot) * (S::STEP_BYTES >> 4);
+                const uint32_t d = utmem + S::O_COL + t * D, p = utmem + S::S_COL + (2 * t + (i & 1)) * S::NS;
+                const int blocks = min(NP, (t ? pages1 : pages0) - i * NP) * (T / 16);    // of 16 tokens
+#pragma unroll
+                for (int kk = 0; kk < S::NS / 16; ++kk)
+                    if (kk < blocks)
+                        tc::mma_f16_ta_warp(d, p + kk * 8, bd + ((kk * 16 / T * S::PAGE_BYTES + kk * 16 % T * 128) >> 4), ID_O,
+                                       i == 0 && kk == 0 ? 0u : 1u);
+                tc::commit_warp(smem_u32(o_done + t));
+                if (!upaired || t == 1) tc::commit_warp(smem_u32(empty + slot));
+            };
+            if (wait_for(q_full, 0) && upaired) wait_for(q_full + 1, 0);
+            for (int j = 0; j < 2 && ok; ++j)
+                for (int t = 0; t < 2 && ok; ++t)
+                    if (j < (t ? un1 : un0)) scores(t, j);
+            for (int i = 0; i < un0 && ok; ++i) {
+                products(0, i, un0);
+                // the next scores overwrite the weights of the step before: its product is long done
+                if (ok && i > 0 && i + 1 < un1 && wait_for(o_done + 1, i - 1)) scores(1, i + 1);
+                if (ok && i < un1) products(1, i, un1);
+                if (ok && i + 2 < un0 && wait_for(o_done, i)) scores(0, i + 2);
+                ok = ok && !__any_sync(kFullMask, *abort_flag != 0);
             }
-            // Paired: positions K0, V0, K1, V1, ..; a step's V and the next step's K are
-            // taken by stream 0 and given back by stream 1, so both are open at once.
-            for (int i = 0; i < n0 && ok; ++i) {
-                const int base = pos;
-                for (int t = 0; t < streams && ok; ++t) {
-                    const int n = t ? n1 : n0;
-                    if (i >= n) continue;
-                    if (paired) pos = base;
-                    const int p0 = it.s(t).first + i * NP;
-                    if (t == 0 || !paired) vb = take();
-                    ok = ok && !*abort_flag && mbar_wait(smem_u32(p_full + t), i & 1);
-                    if (!ok) break;
-                    tc::fence_after_sync();
-                    products(t, vb, min(NP, it.s(t).end - p0) * T, i == 0);
-                    if (!paired || t == streams - 1) give();
-                    else ++pos;
-                    if (i + 1 >= n) continue;
-                    if (t == 0 || !paired) kb = take();
-                    // the next scores overwrite the weights that this product reads
-                    ok = ok && mbar_wait(smem_u32(o_done + t), i & 1);
-                    if (!ok) break;
-                    tc::fence_after_sync();
-                    scores(t, kb);
-                    if (!paired || t == streams - 1) give();
-                    else ++pos;
-                }
-            }
-            if (!ok) fail_wait();
+            if (!ok && lane == 0) fail_wait();
             // every MMA has finished before shared and tensor memory go
-            tc::commit(smem_u32(mma_done));
-            if (!mbar_wait(smem_u32(mma_done), 0)) fail_wait();
+            tc::commit_warp(smem_u32(mma_done));
+            if (!mbar_wait(smem_u32(mma_done), 0) && lane == 0) fail_wait();
         }
         __syncwarp();
     } else {
@@ -294,9 +298,10 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             // the tile's query rows, 16-byte chunks XORed by row % 8 (K-major, 128-byte swizzle)
             constexpr int CPR = D / 8;
             uint8_t *qs = qbuf + t * S::Q_BYTES;
-#pragma unroll 4
-            for (int e = threadIdx.x & 127; e < S::M * CPR; e += 128) {
-                const int row = e / CPR, c = e % CPR, gr = st.tile * S::M + row, member = gr / a.group;
+#pragma unroll
+            for (int j = 0; j < CPR; ++j) {
+                const int e = j * 128 + (threadIdx.x & 127), row = e / CPR, c = e % CPR;
+                const int gr = st.tile * S::M + row, member = gr / a.group;
                 uint4 x = make_uint4(0u, 0u, 0u, 0u);
                 if (member < it.members) {
                     const int64_t b = __ldg(a.members + it.member0 + member);
@@ -310,52 +315,42 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             if (lane == 0) mbar_arrive(smem_u32(q_full + t));
         }
         const uint32_t lanes = uint32_t(32 * quad) << 16;
-        const uint32_t ts = tmem + lanes + S::S_COL + t * S::NS, to = tmem + lanes + S::O_COL + t * D;
+        const uint32_t ts = tmem + lanes + S::S_COL + 2 * t * S::NS, to = tmem + lanes + S::O_COL + t * D;
         const auto warp_wait = [&](uint64_t *bar, int parity) {
             return __all_sync(kFullMask, mbar_wait(smem_u32(bar), uint32_t(parity)));
         };
         float m = -INFINITY;                            // the row's reference
-        unsigned long long l2 = 0;                      // two partial denominators
+        unsigned long long l2 = 0, l3 = 0;              // four partial denominators
         bool ok = true;
         for (int i = 0; i < n; ++i) {
-            if (!warp_wait(s_full + t, i & 1)) {
+            if (!warp_wait(s_full + 2 * t + (i & 1), i >> 1 & 1)) {
                 ok = false;
                 break;
             }
             tc::fence_after_sync();
+            const uint32_t block = ts + (i & 1) * S::NS;
+            uint32_t x[32], y[32];
+            tc::ld_32x32b_x32(block, x);
+            tc::ld_32x32b_x32(block + 32, y);
+            tc::wait_ld();
             // columns past the run's last page hold scores of stale rows
             const int live = min(NP, st.end - st.first - i * NP) * T;
-            uint32_t x[32], y[32];
-            const auto load = [&](uint32_t (&v)[32], int c) { tc::ld_32x32b_x32(ts + 32 * c, v); };
-            const auto mask = [&](uint32_t (&v)[32], int c) {
-                if (live < S::NS)
+            if (live < S::NS) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (32 * c + e >= live) v[e] = __float_as_uint(-INFINITY);
-            };
-            float top0 = -INFINITY, top1 = -INFINITY;
-            const auto raise = [&]() {
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    top0 = max3(top0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-                    top1 = max3(top1, __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+                for (int e = 0; e < 32; ++e) {
+                    if (e >= live) x[e] = __float_as_uint(-INFINITY);
+                    if (32 + e >= live) y[e] = __float_as_uint(-INFINITY);
                 }
-            };
-            // Two passes over the 128 scores, 64 of them held in registers: the upper half is
-            // read twice.  (All 128 at once spill.)
-            load(x, 2);
-            load(y, 3);
-            tc::wait_ld();
-            mask(x, 2);
-            mask(y, 3);
-            raise();
-            load(x, 0);
-            load(y, 1);
-            tc::wait_ld();
-            mask(x, 0);
-            mask(y, 1);
-            raise();
-            const float peak = fmaxf(top0, top1) * a.scale_log2;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                top[0] = max3(top[0], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                top[1] = max3(top[1], __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+                top[2] = max3(top[2], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+                top[3] = max3(top[3], __uint_as_float(y[e + 2]), __uint_as_float(y[e + 3]));
+            }
+            const float peak = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
             const bool moves = peak > m + 15.f;
             if (__any_sync(kFullMask, moves)) {
                 const float next = moves ? peak - 7.f : m;
@@ -376,51 +371,46 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                     }
                     tc::wait_st();
                 }
-                const float2 l = unpack_f32x2(l2);
-                l2 = pack_f32x2(l.x * f, l.y * f);
+                l2 = mul_f32x2(l2, pack_f32x2(f, f));
+                l3 = mul_f32x2(l3, pack_f32x2(f, f));
                 m = next;
             }
             const float base = m == -INFINITY ? 0.f : m;
             const unsigned long long scale2 = pack_f32x2(a.scale_log2, a.scale_log2), base2 = pack_f32x2(-base, -base);
-            // 32 weights into columns [16 c, 16 c + 16), where the scores have been read
-            const auto emit = [&](const uint32_t (&v)[32], int c) {
+            // 32 weights of x or y into columns [16 c, 16 c + 16) of the block
+            const auto emit = [&](const uint32_t (&v)[32], int c, unsigned long long &sum) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float2 z = unpack_f32x2(fma_f32x2(
                         pack_f32x2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, base2));
                     const float w0 = ex2_approx(z.x), w1 = ex2_approx(z.y);
-                    l2 = add_f32x2(l2, pack_f32x2(w0, w1));
+                    sum = add_f32x2(sum, pack_f32x2(w0, w1));
                     p[e] = pack_half2(w0, w1);
                 }
-                tc::st_32x32b_x16(ts + 16 * c, p);
+                tc::st_32x32b_x16(block + 16 * c, p);
             };
-            emit(x, 0);
-            load(x, 2);
-            emit(y, 1);
-            load(y, 3);
-            tc::wait_ld();
-            mask(x, 2);
-            mask(y, 3);
-            emit(x, 2);
-            emit(y, 3);
+            emit(x, 0, l2);
+            emit(y, 1, l3);
             tc::wait_st();
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(p_full + t));
+            if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * t + (i & 1)));
         }
         if (!ok && lane == 0) fail_wait();
         // ------------------------------------------------------------ partial
         if (n > 0 && ok) {
-            ok = warp_wait(o_done + t, (n - 1) & 1);
+            // phase by phase: a parity wait cannot tell a phase from the one two before it
+            ok = (n == 1 || warp_wait(o_done + t, n & 1)) && warp_wait(o_done + t, (n - 1) & 1);
             if (!ok && lane == 0) fail_wait();
         }
         if (n > 0 && ok) {
             tc::fence_after_sync();
-            const float2 l = unpack_f32x2(l2);
-            const int64_t row = int64_t(st.slot) * S::M + r;
+            // partials lie [D / 8][rows][8]: a warp's stores are dense, and a row's reads whole sectors
+            const float2 l = unpack_f32x2(add_f32x2(l2, l3));
             const bool on = (st.tile * S::M + r) / a.group < it.members;
-            float *dst = a.part_o + row * D;
+            float *dst = a.part_o + (int64_t(st.slot) * D * S::M + r * 8);
+#pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tc::ld_32x32b_x32(to + c, o);
@@ -428,9 +418,10 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 if (on)
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        *reinterpret_cast<uint4 *>(dst + (c + e) / 8 * (S::M * 8) + e % 8) =
+                            make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
-            if (on) a.part_ml[row] = make_float2(m, l.x + l.y);
+            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, l.x + l.y);
             tc::fence_before_sync();
         }
     }
