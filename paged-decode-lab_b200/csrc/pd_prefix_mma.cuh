@@ -7,15 +7,15 @@
 //   * split: one row tile whose pages are cut in two runs; each stream loads
 //     its own steps (few rows: the prefix's bytes bound the kernel, and two
 //     streams keep both the loads and the softmax busy).
-// Roles (10 warps):
+// Roles (11 warps):
 //   * warps 0-3 / 4-7: softmax of stream 0 / 1, one thread per query row
 //     (tensor-memory lane).  S is read from tensor memory, the weights go back
 //     as FP16 over the scores' own columns, where the PV product reads them as
 //     its A operand;
-//   * warp 8, two lanes: TMA loads of K and V steps into one ring (one lane its
-//     even slots, one its odd slots), one box per page;
-//   * warp 9, one elected lane: the MMAs.  S = Q K^T (M 128, N 64), O += P V (M 128,
-//     N = head dim).
+//   * warp 8, one elected lane: TMA loads of K and V steps into one ring, one box
+//     per page;
+//   * warps 9 / 10, one elected lane each: the MMAs of stream 0 / 1.  S = Q K^T
+//     (M 128, N 64), O += P V (M 128, N = head dim).
 // Each stream has two score blocks, so that a softmax finds its next scores
 // ready: those of step i + 2 are issued once the PV product of step i, whose
 // weights lie in the same block, has completed.  (Steps of 128 tokens leave
@@ -50,16 +50,16 @@ struct PrefixShape {
     static constexpr int STEP_BYTES = NP * PAGE_BYTES;
     static constexpr int Q_BOX = M * 128;
     static constexpr int Q_BYTES = NBOX * Q_BOX;
-    static constexpr int SLOTS = D == 128 ? 10 : 16;    // ring slots of one K or V step; even: a lane's slots stay its own
+    static constexpr int K_SLOTS = D == 128 ? 2 : 4, V_SLOTS = D == 128 ? 3 : 4;   // of one step, per stream
+    static constexpr int SLOTS = 2 * (K_SLOTS + V_SLOTS);
     static constexpr int SOFTMAX_WARPS = 8, W_LOAD = 8, W_MMA = 9;
-    static constexpr int THREADS = 320;
+    static constexpr int THREADS = 352;                 // W_MMA + t issues stream t's MMAs
     // tensor memory: score blocks (weights in their first half) [stream][2], outputs [stream]
     static constexpr int S_COL = 0, O_COL = 4 * NS;
     static constexpr int TMEM_COLS = 512;
     static constexpr int NBARS = 2 * SLOTS + 2 + 4 + 4 + 2 + 1;
     static constexpr size_t SMEM = 1024 + 2 * size_t(Q_BYTES) + size_t(SLOTS) * STEP_BYTES + NBARS * 8 + 16;
     static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory budget");
-    static_assert(SLOTS % 2 == 0, "a slot belongs to one lane");
     static_assert(SMEM <= 232448 && SMEM > 116 * 1024, "one CTA per SM: tensor memory is never contended");
 };
 
@@ -101,26 +101,29 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixArgs &a, int i) {
     return it;
 }
 
-// The order in which the MMA thread first uses the ring: use(position, stream,
-// is_v, step) for each.  Paired streams share stream 0's steps.
-template <typename Use>
-__device__ __forceinline__ void ring_order(int n0, int n1, bool paired, Use use) {
-    if (paired) n1 = 0;
-    int pos = 0;
-    for (int i = 0; i < 2; ++i) {
-        if (i < n0 && !use(pos++, 0, false, i)) return;
-        if (i < n1 && !use(pos++, 1, false, i)) return;
+// Cursor over a run of ring slots; `phase` is the parity of the slot's current use.
+struct RingCursor {
+    int first, count, slot, phase;
+    __device__ __forceinline__ void next() {
+        if (++slot == first + count) {
+            slot = first;
+            phase ^= 1;
+        }
     }
-    for (int i = 0; i < n0; ++i) {
-        if (!use(pos++, 0, true, i)) return;
-        if (i > 0 && i + 1 < n1 && !use(pos++, 1, false, i + 1)) return;
-        if (i < n1 && !use(pos++, 1, true, i)) return;
-        if (i + 2 < n0 && !use(pos++, 0, false, i + 2)) return;
-    }
+};
+
+// K and V steps have slots of their own: paired streams share 2 K_SLOTS and 2
+// V_SLOTS of them, split streams have half each.
+template <typename S>
+__device__ __forceinline__ RingCursor k_cursor(int t, bool paired) {
+    const int first = paired ? 0 : t * S::K_SLOTS;
+    return RingCursor{first, paired ? 2 * S::K_SLOTS : S::K_SLOTS, first, 0};
 }
-// Paired: the positions of K step j and V step i of n.
-__device__ __forceinline__ int paired_k(int j) { return j < 2 ? j : 2 * j - 1; }
-__device__ __forceinline__ int paired_v(int i, int n) { return min(n, 2) + i + min(i, max(n - 2, 0)); }
+template <typename S>
+__device__ __forceinline__ RingCursor v_cursor(int t, bool paired) {
+    const int first = 2 * S::K_SLOTS + (paired ? 0 : t * S::V_SLOTS);
+    return RingCursor{first, paired ? 2 * S::V_SLOTS : S::V_SLOTS, first, 0};
+}
 
 template <int D, int T>
 __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
@@ -143,10 +146,16 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1) + 1;
 
     const int warp = int(__reduce_max_sync(kFullMask, threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    const PrefixItem it = prefix_item(a, blockIdx.x);
+    const int n0 = it.s0.steps(NP), n1 = it.s1.steps(NP);   // n1 <= n0; paired: n1 == n0
+    const bool paired = it.paired != 0;
+    // Warps 8 to 10 stay converged, and what they hand to the hardware is the same in all lanes
+    // (reductions over the warp give the compiler the proof): operands then live in uniform registers.
+    const auto uniform = [](int x) { return __reduce_max_sync(kFullMask, x); };
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
             mbar_init(smem_u32(full + s), 1);
-            mbar_init(smem_u32(empty + s), 1);
+            mbar_init(smem_u32(empty + s), 1 + (it.paired ? 1 : 0));   // a commit per stream that reads it
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(smem_u32(q_full + t), 4);
@@ -156,7 +165,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 mbar_init(smem_u32(p_full + 2 * t + b), 4);
             }
         }
-        mbar_init(smem_u32(mma_done), 1);
+        mbar_init(smem_u32(mma_done), 2);
         *abort_flag = 0;
         mbar_init_fence();
     }
@@ -165,9 +174,6 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         tc::relinquish_alloc_permit();
         tc::fence_before_sync();
     }
-    const PrefixItem it = prefix_item(a, blockIdx.x);
-    const int n0 = it.s0.steps(NP), n1 = it.s1.steps(NP);   // n1 <= n0; paired: n1 == n0
-    const bool paired = it.paired != 0;
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
@@ -182,112 +188,127 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
 
     if (warp == S::W_LOAD) {
         // ------------------------------------------------------------ loads
-        if (lane < 2) {
-            tma_prefetch_descriptor(lane == 0 ? &tm_k : &tm_v);
-            int last = -1;              // the last position this lane loaded
-            ring_order(n0, n1, paired, [&](int pos, int t, bool is_v, int step) {
-                if ((pos & 1) != lane) return true;
-                const int p0 = it.s(t).first + step * NP, n = min(NP, it.s(t).end - p0);
-                int ids[NP];
+        const bool upaired = uniform(it.paired) != 0;
+        const int un0 = uniform(n0), un1 = upaired ? 0 : uniform(n1);
+        const int first0 = uniform(it.s0.first), end0 = uniform(it.s0.end);
+        const int first1 = uniform(it.s1.first), end1 = uniform(it.s1.end);
+        const int head = uniform(it.head);
+        // one of the four sequences of steps: K or V of a stream, with page ids 32 at a time, one per lane
+        struct Feed {
+            RingCursor at;
+            int window = 0, base = -64, steps = 0;
+        };
+        Feed k0{k_cursor<S>(0, upaired)}, k1{k_cursor<S>(1, upaired)}, v0{v_cursor<S>(0, upaired)},
+            v1{v_cursor<S>(1, upaired)};
+        bool ok = true;
+        const auto load = [&](Feed &f, int first, int end, bool is_v) {
+            const int p0 = first + f.steps * NP, n = min(NP, end - p0);
+            if (p0 + NP > f.base + 32) {
+                f.base = p0;
+                f.window = p0 + lane < end ? __ldg(a.pages + it.page0 + p0 + lane) : 0;
+            }
+            // (a fresh barrier's preceding phase counts as complete: the first pass does not wait)
+            ok = __all_sync(kFullMask, mbar_wait(smem_u32(empty + f.at.slot), uint32_t(f.at.phase ^ 1))) &&
+                 !__any_sync(kFullMask, *abort_flag != 0);
+            if (!ok) return;
+            const uint32_t bar = smem_u32(full + f.at.slot);
+            const uint32_t dst = smem_u32(ring) + uint32_t(f.at.slot) * S::STEP_BYTES;
+            if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(n) * S::PAGE_BYTES);
+            __syncwarp();
 #pragma unroll
-                for (int p = 0; p < NP; ++p) ids[p] = p < n ? __ldg(a.pages + it.page0 + p0 + p) : 0;
-                const int slot = pos % SLOTS, use = pos / SLOTS;
-                if (use > 0) {      // both lanes are of one warp: poll without suspending it
-                    const unsigned long long t0 = global_ns();
-                    while (!mbar_test_wait(smem_u32(empty + slot), (use - 1) & 1)) {
-                        if (*abort_flag) return false;
-                        if (global_ns() - t0 > kWaitTimeoutNs) {
-                            fail_wait();
-                            return false;
-                        }
-                    }
-                }
-                last = pos;
-                const uint32_t bar = smem_u32(full + slot), dst = smem_u32(ring + size_t(slot) * S::STEP_BYTES);
-                mbar_arrive_expect_tx(bar, uint32_t(n) * S::PAGE_BYTES);
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    if (p >= n) continue;
-                    if (is_v) tma_load_5d(dst + p * S::PAGE_BYTES, &tm_v, 0, 0, 0, it.head, ids[p], bar);
-                    else tma_load_5d(dst + p * S::PAGE_BYTES, &tm_k, 0, 0, it.head * S::NBOX, 0, ids[p], bar);
-                }
-                return true;
-            });
-            // no copy of this lane is in flight when the CTA ends, whatever became of its readers
-            for (int pos = last; pos >= 0 && pos > last - SLOTS; pos -= 2)
-                if (!mbar_wait(smem_u32(full + pos % SLOTS), (pos / SLOTS) & 1)) fail_wait();
+            for (int p = 0; p < NP; ++p) {
+                if (p >= n) continue;
+                const int id = uniform(__shfl_sync(kFullMask, f.window, p0 - f.base + p));
+                if (is_v) tma_load_5d_warp(dst + p * S::PAGE_BYTES, &tm_v, 0, 0, 0, head, id, bar);
+                else tma_load_5d_warp(dst + p * S::PAGE_BYTES, &tm_k, 0, 0, head * S::NBOX, 0, id, bar);
+            }
+            f.at.next();
+            ++f.steps;
+        };
+        // K steps 0 and 1, then V step i and K step i + 2
+        for (int j = -2; j < un0 && ok; ++j) {
+            if (j >= 0) load(v0, first0, end0, true);
+            if (ok && j >= 0 && j < un1) load(v1, first1, end1, true);
+            if (ok && j + 2 < un0) load(k0, first0, end0, false);
+            if (ok && j + 2 < un1) load(k1, first1, end1, false);
         }
+        if (!ok && lane == 0) fail_wait();
+        // no copy is in flight when the CTA ends, whatever became of its readers
+        const auto drain = [&](const Feed &f) {
+            for (int i = 0; i < min(f.at.count, f.steps); ++i) {
+                const int slot = f.at.first + i;
+                const int phase = slot < f.at.slot ? f.at.phase : f.at.phase ^ 1;    // of its last use
+                if (!mbar_wait(smem_u32(full + slot), uint32_t(phase)) && lane == 0) fail_wait();
+            }
+        };
+        drain(k0);
+        drain(k1);
+        drain(v0);
+        drain(v1);
         __syncwarp();
-    } else if (warp == S::W_MMA) {
-        // ------------------------------------------------------------ MMAs (one elected lane)
-        {
-            // The warp stays converged and every operand is the same in all lanes (reductions over
-            // the warp give the compiler the proof), so that they live in uniform registers.
-            const auto uniform = [](int x) { return __reduce_max_sync(kFullMask, x); };
-            const int un0 = uniform(n0), un1 = uniform(n1);
-            const int pages0 = uniform(it.s0.end - it.s0.first), pages1 = uniform(it.s1.end - it.s1.first);
-            const bool upaired = uniform(it.paired) != 0;
-            const uint32_t utmem = __reduce_max_sync(kFullMask, tmem);
-            constexpr uint32_t ID_S = tc::idesc_f16_f32(S::M, S::NS, false, false);   // Q, K: K-major
-            constexpr uint32_t ID_O = tc::idesc_f16_f32(S::M, D, false, true);        // V: MN-major
-            const uint64_t q_desc = tc::smem_desc(smem_u32(qbuf), 16, 1024, tc::kSwizzle128);
-            const uint64_t k_desc = tc::smem_desc(smem_u32(ring), 16, S::NBOX * 1024, tc::kSwizzle128);
-            const uint64_t v_desc = tc::smem_desc(smem_u32(ring), T * 128, 1024, tc::kSwizzle128);
-            bool ok = true;
-            int pos = 0;                // split streams: ring positions used
-            const auto wait_for = [&](uint64_t *bar, int phase) {
-                ok = ok && __all_sync(kFullMask, mbar_wait(smem_u32(bar), uint32_t(phase & 1)));
-                return ok;
-            };
-            // S of step j of stream t into its block j % 2
-            const auto scores = [&](int t, int j) {
-                const int at = upaired ? paired_k(j) : pos++, slot = at % SLOTS;
-                if ((t == 0 || !upaired) && !wait_for(full + slot, at / SLOTS)) return;
-                tc::fence_after_sync();
-                const uint64_t ad = q_desc + (upaired && t ? S::Q_BYTES >> 4 : 0);
-                const uint64_t bd = k_desc + uint32_t(slot) * (S::STEP_BYTES >> 4);
-                const uint32_t d = utmem + S::S_COL + (2 * t + (j & 1)) * S::NS;
+    } else if (warp >= S::W_MMA) {
+        // ------------------------------------------------------------ MMAs of one stream (one elected lane)
+        const int t = warp - S::W_MMA;
+        const bool upaired = uniform(it.paired) != 0;
+        const int un = uniform(t ? n1 : n0);
+        const int pages = uniform(t ? it.s1.end - it.s1.first : it.s0.end - it.s0.first);
+        const uint32_t utmem = __reduce_max_sync(kFullMask, tmem);
+        constexpr uint32_t ID_S = tc::idesc_f16_f32(S::M, S::NS, false, false);   // Q, K: K-major
+        constexpr uint32_t ID_O = tc::idesc_f16_f32(S::M, D, false, true);        // V: MN-major
+        const uint64_t q_desc =
+            tc::smem_desc(smem_u32(qbuf) + (upaired && t ? S::Q_BYTES : 0), 16, 1024, tc::kSwizzle128);
+        const uint64_t k_desc = tc::smem_desc(smem_u32(ring), 16, S::NBOX * 1024, tc::kSwizzle128);
+        const uint64_t v_desc = tc::smem_desc(smem_u32(ring), T * 128, 1024, tc::kSwizzle128);
+        const uint32_t s_block = utmem + S::S_COL + 2 * t * S::NS, o_block = utmem + S::O_COL + t * D;
+        RingCursor kr = k_cursor<S>(t, upaired), vr = v_cursor<S>(t, upaired);
+        bool ok = true;
+        const auto wait_for = [&](uint64_t *bar, int phase) {
+            ok = ok && __all_sync(kFullMask, mbar_wait(smem_u32(bar), uint32_t(phase & 1)));
+        };
+        // scores of step j into block j % 2
+        const auto scores = [&](int j) {
+            wait_for(full + kr.slot, kr.phase);
+            if (!ok) return;
+            tc::fence_after_sync();
+            const uint64_t bd = k_desc + uint32_t(kr.slot) * (S::STEP_BYTES >> 4);
+            const uint32_t d = s_block + (j & 1) * S::NS;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                    tc::mma_f16_warp(d, ad + (((kk >> 2) * S::Q_BOX + (kk & 3) * 32) >> 4),
-                                bd + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), ID_S, kk > 0 ? 1u : 0u);
-                tc::commit_warp(smem_u32(s_full + 2 * t + (j & 1)));
-                if (!upaired || t == 1) tc::commit_warp(smem_u32(empty + slot));
-            };
-            // O += P V of step i of stream t
-            const auto products = [&](int t, int i, int n) {
-                const int at = upaired ? paired_v(i, n) : pos++, slot = at % SLOTS;
-                if ((t == 0 || !upaired) && !wait_for(full + slot, at / SLOTS)) return;
-                if (!wait_for(p_full + 2 * t + (i & 1), i >> 1)) return;
-                tc::fence_after_sync();
-                const uint64_t bd = v_desc + uint32_t(slot) * (S::STEP_BYTES >> 4);
-                const uint32_t d = utmem + S::O_COL + t * D, p = utmem + S::S_COL + (2 * t + (i & 1)) * S::NS;
-                const int blocks = min(NP, (t ? pages1 : pages0) - i * NP) * (T / 16);    // of 16 tokens
+            for (int kk = 0; kk < D / 16; ++kk)
+                tc::mma_f16_warp(d, q_desc + (((kk >> 2) * S::Q_BOX + (kk & 3) * 32) >> 4),
+                                 bd + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), ID_S, kk > 0 ? 1u : 0u);
+            tc::commit_warp(smem_u32(s_full + 2 * t + (j & 1)));
+            tc::commit_warp(smem_u32(empty + kr.slot));
+            kr.next();
+        };
+        if (un > 0) wait_for(q_full + (upaired ? t : 0), 0);
+        for (int j = 0; j < min(un, 2) && ok; ++j) scores(j);
+        for (int i = 0; i < un && ok; ++i) {
+            wait_for(full + vr.slot, vr.phase);
+            wait_for(p_full + 2 * t + (i & 1), i >> 1);
+            if (!ok) break;
+            tc::fence_after_sync();
+            const uint64_t bd = v_desc + uint32_t(vr.slot) * (S::STEP_BYTES >> 4);
+            const uint32_t p = s_block + (i & 1) * S::NS;
+            const int blocks = min(NP, pages - i * NP) * (T / 16);    // of 16 tokens
 #pragma unroll
-                for (int kk = 0; kk < S::NS / 16; ++kk)
-                    if (kk < blocks)
-                        tc::mma_f16_ta_warp(d, p + kk * 8, bd + ((kk * 16 / T * S::PAGE_BYTES + kk * 16 % T * 128) >> 4), ID_O,
-                                       i == 0 && kk == 0 ? 0u : 1u);
-                tc::commit_warp(smem_u32(o_done + t));
-                if (!upaired || t == 1) tc::commit_warp(smem_u32(empty + slot));
-            };
-            if (wait_for(q_full, 0) && upaired) wait_for(q_full + 1, 0);
-            for (int j = 0; j < 2 && ok; ++j)
-                for (int t = 0; t < 2 && ok; ++t)
-                    if (j < (t ? un1 : un0)) scores(t, j);
-            for (int i = 0; i < un0 && ok; ++i) {
-                products(0, i, un0);
-                // the next scores overwrite the weights of the step before: its product is long done
-                if (ok && i > 0 && i + 1 < un1 && wait_for(o_done + 1, i - 1)) scores(1, i + 1);
-                if (ok && i < un1) products(1, i, un1);
-                if (ok && i + 2 < un0 && wait_for(o_done, i)) scores(0, i + 2);
+            for (int kk = 0; kk < S::NS / 16; ++kk)
+                if (kk < blocks)
+                    tc::mma_f16_ta_warp(o_block, p + kk * 8,
+                                        bd + ((kk * 16 / T * S::PAGE_BYTES + kk * 16 % T * 128) >> 4), ID_O,
+                                        i == 0 && kk == 0 ? 0u : 1u);
+            tc::commit_warp(smem_u32(o_done + t));
+            tc::commit_warp(smem_u32(empty + vr.slot));
+            vr.next();
+            if (i + 2 < un) {
+                wait_for(o_done + t, i);    // the next scores overwrite this step's weights
+                if (ok) scores(i + 2);
                 ok = ok && !__any_sync(kFullMask, *abort_flag != 0);
             }
-            if (!ok && lane == 0) fail_wait();
-            // every MMA has finished before shared and tensor memory go
-            tc::commit_warp(smem_u32(mma_done));
-            if (!mbar_wait(smem_u32(mma_done), 0) && lane == 0) fail_wait();
         }
+        if (!ok && lane == 0) fail_wait();
+        // every MMA has finished before shared and tensor memory go
+        tc::commit_warp(smem_u32(mma_done));
+        if (!mbar_wait(smem_u32(mma_done), 0) && lane == 0) fail_wait();
         __syncwarp();
     } else {
         // ------------------------------------------------------------ softmax, one thread per row
