@@ -127,8 +127,9 @@ struct SimtShape {
 // streams (see pd_prefix_mma.cuh).
 struct MmaShape {
     static constexpr int64_t rows = 128, step_tokens = 64;
-    // start and end of a CTA (launch, first loads, the partials' store), in steps
-    static constexpr int64_t overhead_steps = 8;
+    // in steps: start and end of a CTA (launch, first loads, rows out), and the partials' way through
+    // the merge kernel
+    static constexpr int64_t overhead_steps = 7, merge_steps = 10;
 };
 
 }  // namespace
@@ -145,12 +146,20 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
         return (int64_t(g.members.size()) * p.group + p.tile_rows - 1) / p.tile_rows;
     };
     const auto steps_of = [&](const PrefixGroup &g) { return (g.pages + step_pages - 1) / step_pages; };
-    // Steps per work item: FP16 takes what finishes first when the CTAs run in
-    // waves of one per SM and each costs its steps and the fixed overhead.
+    // FP16: what finishes first when the CTAs run in waves of one per SM and each
+    // costs its steps and the fixed overhead: a CTA per pair of row tiles or per tile
+    // that sees the whole prefix and writes the output (direct), or any number of
+    // pieces that leave partials for the merge kernel.
     int64_t item_steps = 1;
+    bool pair_tiles = true;
+    p.direct = false;
     if (mma) {
-        int64_t most = 1, best = INT64_MAX;
-        for (const PrefixGroup &g : p.groups) most = std::max<int64_t>(most, steps_of(g));
+        int64_t most = 1, pairs = 0, tiles = 0, best = INT64_MAX;
+        for (const PrefixGroup &g : p.groups) {
+            most = std::max<int64_t>(most, steps_of(g));
+            pairs += L.kv_heads * ((tiles_of(g) + 1) / 2);
+            tiles += L.kv_heads * tiles_of(g);
+        }
         const auto items = [&](int64_t steps) {
             int64_t n = 0;
             for (const PrefixGroup &g : p.groups) {
@@ -159,10 +168,17 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
             }
             return n;
         };
+        const auto waves = [&](int64_t ctas) { return (ctas + sm_count - 1) / sm_count; };
         for (int64_t steps = 1; steps <= most; ++steps) {
-            const int64_t waves = (items(steps) + sm_count - 1) / sm_count;
-            const int64_t cost = waves * (MmaShape::overhead_steps + steps);
+            const int64_t cost = waves(items(steps)) * (MmaShape::overhead_steps + steps) + MmaShape::merge_steps;
             if (cost < best) best = cost, item_steps = steps;
+        }
+        const int64_t by_pair = waves(pairs) * (MmaShape::overhead_steps + most);
+        const int64_t by_tile = waves(tiles) * (MmaShape::overhead_steps + (most + 1) / 2);
+        if (by_pair <= best || by_tile <= best) {
+            p.direct = !p.groups.empty();
+            pair_tiles = by_pair <= by_tile;
+            item_steps = most;
         }
     } else {
         int64_t work = 0;
@@ -194,7 +210,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
         };
         for (int h = 0; h < L.kv_heads; ++h) {
             for (int64_t t = 0; t < ntiles; ++t) {
-                const bool paired = mma && (t ^ 1) < ntiles;
+                const bool paired = mma && pair_tiles && (t ^ 1) < ntiles;
                 const bool split = mma && !paired && steps > 1;
                 int64_t pieces = (steps + item_steps - 1) / item_steps;
                 if (split) pieces = (steps + 2 * item_steps - 1) / (2 * item_steps) * 2;
@@ -219,13 +235,14 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
                                 std::swap(sx, sy);
                             }
                         }
-                        p.items.insert(p.items.end(), {m0, n, h, 0, pg, 0, 0, 0, tile, x[0], x[1], sx, tile, x[2], x[3], sy});
+                        p.items.insert(p.items.end(), {m0, n, h, 0, pg, g.pages, 0, 0, tile, x[0], x[1], sx, tile, x[2],
+                                                       x[3], sy});
                     }
                 } else if (t % 2) {
                     // both tiles of a pair have the same pieces; this one's slots follow the other's
                     for (int64_t c = 0; c < pieces; ++c)
                         p.items.insert(p.items.end(),
-                                       {m0, n, h, 1, pg, 0, 0, 0, tile - 1, bound(c, pieces), bound(c + 1, pieces),
+                                       {m0, n, h, 1, pg, g.pages, 0, 0, tile - 1, bound(c, pieces), bound(c + 1, pieces),
                                         int32_t(slot - pieces + c), tile, bound(c, pieces), bound(c + 1, pieces),
                                         int32_t(slot + c)});
                 }
@@ -234,6 +251,17 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
         members.insert(members.end(), g.members.begin(), g.members.end());
         const int32_t *row = table + int64_t(g.members[0]) * p.width;
         pages.insert(pages.end(), row, row + g.pages);
+    }
+    if (p.direct) {
+        // every row is written by the prefix kernel: sequences of no group, four to a CTA
+        slots = 0;
+        const size_t first = members.size();
+        for (int b = 0; b < L.batch; ++b)
+            if (p.seqs[size_t(b) * 8] < 0) members.push_back(b);
+        for (size_t at = first; at < members.size(); at += 4) {
+            p.items.insert(p.items.end(), {int32_t(at), int32_t(std::min<size_t>(4, members.size() - at)), 0, 2});
+            p.items.insert(p.items.end(), 12, 0);
+        }
     }
     p.slots = int32_t(slots);
     // Merge: at most four pieces (one batch of loads) per thread set, while the

@@ -15,6 +15,7 @@
 #include "pd_device.cuh"
 #include "pd_prefix.hpp"
 #include "pd_prefix_args.cuh"
+#include "pd_prefix_merge.cuh"
 #include "pd_prefix_mma.cuh"
 
 #define PD_API extern "C" __attribute__((visibility("default")))
@@ -129,64 +130,6 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// (m, l) of one row over the first `limit` tokens of its prefix, and in `o`
-// eight dims of it: for a dynamic launch's sequence that ends inside its prefix,
-// whose row in the group's matrix covers the whole prefix.  D / 8 neighbouring
-// lanes, a token at a time: such lengths are rare, and most of them 0.
-template <typename Elt, int D>
-__device__ __noinline__ float2 prefix_row(const PrefixArgs &a, int64_t row, int kv_head, const int32_t *pages,
-                                          int limit, int lane, float (&o)[8]) {
-    constexpr int LANES = D / 8;
-    const unsigned mates = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
-    float q[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        q[i] = float(static_cast<const Elt *>(a.q)[row * D + lane * 8 + i]) * a.scale_log2;
-        o[i] = 0.f;
-    }
-    for (int t = 0; t < limit; ++t) {
-        const int64_t at = ((int64_t(pages[t / a.page_size]) * a.page_size + t % a.page_size) * a.Hkv + kv_head) * D +
-                           lane * 8;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(q[i], float(static_cast<const Elt *>(a.k)[at + i]), s);
-#pragma unroll
-        for (int x = LANES / 2; x > 0; x >>= 1) s += __shfl_xor_sync(mates, s, x);
-        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-        const float shrink = exp2f(m - base), p = exp2f(s - base);
-        l = fmaf(l, shrink, p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], shrink, p * float(static_cast<const Elt *>(a.v)[at + i]));
-        m = top;
-    }
-    return make_float2(m, l);
-}
-
-// Eight FP32 values to eight elements, one rounding each.
-__device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
-    *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4 *>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void store8(__half *dst, const float (&x)[8]) {
-    *reinterpret_cast<uint4 *>(dst) =
-        make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
-}
-
-// A part of a row: softmax statistics and this thread's eight dims, o not normalised.
-struct RowPart {
-    float m = -INFINITY, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    // Take in (m2, l2, x).  Parts without a token have l2 = 0; a NaN denominator stays one.
-    __device__ __forceinline__ void absorb(float m2, float l2, const float (&x)[8]) {
-        if (l2 == 0.f) return;
-        const float top = fmaxf(m, m2);
-        const float f = m == top ? 1.f : exp2f(m - top), g = exp2f(m2 - top);
-        l = fmaf(l, f, l2 * g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], f, x[i] * g);
-        m = top;
-    }
-};
-
 // Each output row from the suffix's normalised row and the prefix pieces: D / 8
 // threads per row, eight dims each, and `ways` such sets per row that take every
 // ways-th piece (several where rows are few and pieces many); the sets' parts are
@@ -196,11 +139,11 @@ constexpr int kMergeThreads = 256;
 template <typename Elt, int D>
 __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const PrefixArgs a, int ways) {
     constexpr int LANES = D / 8, BATCH = 4;
-    __shared__ RowPart parts[kMergeThreads];
+    __shared__ float sums[kMergeThreads][10];
     const int per_cta = kMergeThreads / LANES / ways;
     const int set = threadIdx.x / LANES, way = set % ways, lane = threadIdx.x % LANES;
     const int64_t out_row = int64_t(blockIdx.x) * per_cta + set / ways;
-    const bool on = out_row < int64_t(a.B) * a.Hq;
+    bool on = out_row < int64_t(a.B) * a.Hq;
     const int b = on ? int(out_row / a.Hq) : 0, head = int(out_row % a.Hq);
     const int4 sq = on ? __ldg(a.seqs + 2 * b) : make_int4(-1, 0, 0, 0);
     int pieces = 0, prefix_pages = 0;
@@ -215,27 +158,18 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const Prefi
         po += int64_t(tile.x) * a.tile_rows * D + lane * (a.tile_rows * 8) + row % a.tile_rows * 8;
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    RowPart part;
     // a dynamic launch's sequence that ends inside its prefix
-    const bool inside = sizeof(Elt) == 2 && prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size;
-    if (inside) pieces = 0;
-    if (way == 0 && on) {
-        float2 suffix = make_float2(-INFINITY, 0.f);
-        if (a.rows) suffix = __ldcg(reinterpret_cast<const float2 *>(a.stats) + out_row);
-        if (suffix.y != 0.f) {
-            const float4 *x = reinterpret_cast<const float4 *>(a.rows + out_row * D + lane * 8);
-            const float4 u = __ldcg(x), v = __ldcg(x + 1);
-            const float o[8] = {u.x * suffix.y, u.y * suffix.y, u.z * suffix.y, u.w * suffix.y,
-                                v.x * suffix.y, v.y * suffix.y, v.z * suffix.y, v.w * suffix.y};
-            part.absorb(suffix.x, suffix.y, o);
-        }
-        if (inside) {
-            float o[8];
-            const float2 own = prefix_row<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, __ldcg(a.lengths + b), lane, o);
-            part.absorb(own.x, own.y, o);
-        }
+    if (sizeof(Elt) == 2 && prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size) {
+        if (way == 0) row_inside<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, b, lane);
+        pieces = 0;
+        on = false;
     }
     const int64_t ml_step = a.tile_rows, o_step = int64_t(a.tile_rows) * D;
+    const float2 suffix = on && way == 0 ? suffix_stats(a, out_row) : make_float2(-INFINITY, 0.f);
+    float top = top_of(suffix);
+    for (int p = way; p < pieces; p += ways) top = fmaxf(top, top_of(__ldcg(ml + p * ml_step)));
+    RowSum sum(top);
+    add_suffix<D>(sum, a, suffix, out_row, lane);
     for (int p0 = way; p0 < pieces; p0 += ways * BATCH) {
         float2 st[BATCH];
         float4 u[BATCH], v[BATCH];
@@ -251,25 +185,25 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const Prefi
             }
         }
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-            const float o[8] = {u[j].x, u[j].y, u[j].z, u[j].w, v[j].x, v[j].y, v[j].z, v[j].w};
-            part.absorb(st[j].x, st[j].y, o);
-        }
+        for (int j = 0; j < BATCH; ++j) sum.add(st[j], u[j], v[j]);
     }
     if (ways > 1) {
-        parts[threadIdx.x] = part;
+        float *mine = sums[threadIdx.x];
+        mine[0] = sum.top, mine[1] = sum.den;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[2 + i] = sum.o[i];
         __syncthreads();
         if (way != 0) return;
-        for (int w = 1; w < ways; ++w) {
-            const RowPart other = parts[threadIdx.x + w * LANES];
-            part.absorb(other.m, other.l, other.o);
+        float all = -INFINITY;
+        for (int w = 0; w < ways; ++w)
+            if (sums[threadIdx.x + w * LANES][1] != 0.f) all = fmaxf(all, sums[threadIdx.x + w * LANES][0]);
+        sum = RowSum(all);
+        for (int w = 0; w < ways; ++w) {
+            const float *x = sums[threadIdx.x + w * LANES];
+            sum.add(make_float2(x[0], x[1]), make_float4(x[2], x[3], x[4], x[5]), make_float4(x[6], x[7], x[8], x[9]));
         }
     }
-    if (!on) return;
-    const float inv = part.l != 0.f ? 1.f / part.l : 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) part.o[i] *= inv;
-    store8(static_cast<Elt *>(a.out) + out_row * D + lane * 8, part.o);
+    if (on) store_row<Elt, D>(sum, a, out_row, lane);
 }
 
 template <typename... Params, typename... Args>
@@ -311,6 +245,7 @@ cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CU
     if (items && p.dtype == PD_FLOAT16) {
         const MmaEntry e = mma_entry_for(p.layout);
         err = launch_dependent(e.kernel, items, e.threads, e.smem, stream, map_k, map_v, a);
+        if (p.direct) return err;
     } else if (items) {
         err = launch_dependent(prefix_simt_kernel<float, D>, items, kSimtThreads, 0, stream, a);
     }
@@ -357,6 +292,7 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.group = p->group;
     a.page_size = p->layout.page_size;
     a.tile_rows = p->tile_rows;
+    a.direct = p->direct ? 1 : 0;
     a.P = p->layout.physical_pages;
     a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(p->layout.head_dim)));
     pd_status s = PD_OK;

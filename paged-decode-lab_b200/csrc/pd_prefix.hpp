@@ -34,6 +34,7 @@ struct pd_prefix_plan {
     int32_t group = 0;              // G = Hq / Hkv
     int32_t tile_rows = 0;          // query rows of one prefix tile
     int32_t slots = 0;              // partial slots (tile pieces)
+    bool direct = false;            // FP16: the prefix kernel writes the output, no partials or merge kernel
     int32_t merge_ways = 1;         // thread sets that share a row's pieces in the merge
     bool dynamic = false;
     bool suffix_empty = false;      // no sequence has pages past its prefix: nothing for the decode kernel
