@@ -264,6 +264,8 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t v) {
 }
 
 // ---------------------------------------------------------------- pairs of FP32 values
+using f32x2 = unsigned long long;
+
 __device__ __forceinline__ unsigned long long pack_f32x2(float a, float b) {
     unsigned long long r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));

@@ -117,19 +117,19 @@ pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int
 
 namespace {
 
-// FP32 (CUDA cores): tiles of 16 rows, pieces of whole 32-token steps, about
-// four CTAs per SM in all.
-struct SimtShape {
-    static constexpr int64_t rows = 16, step_tokens = 32, ctas_per_sm = 4;
+// FP32 (CUDA cores): tiles of 16 rows, or of 64 where a group has more than 32,
+// 32-token steps, about as many CTAs as are resident at once.
+struct SimtPlan {
+    static constexpr int64_t step_tokens = 32;
 };
 
 // FP16 (tcgen05): tiles of 128 rows, 64-token steps, one CTA per SM with two
 // streams (see pd_prefix_mma.cuh).
 struct MmaShape {
     static constexpr int64_t rows = 128, step_tokens = 64;
-    // in steps: start and end of a CTA (launch, first loads, rows out), and the partials' way through
-    // the merge kernel
-    static constexpr int64_t overhead_steps = 7, merge_steps = 10;
+    // In steps (0.9 us): start and end of a CTA (launch, first loads, rows out); the merge kernel; and
+    // the partials' way through memory, FP32 values a step.
+    static constexpr int64_t overhead_steps = 7, merge_steps = 3, values_per_step = 20 * 128 * 128;
 };
 
 }  // namespace
@@ -139,9 +139,12 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     const int D = L.head_dim;
     const bool mma = p.dtype == PD_FLOAT16;
     p.group = L.query_heads / L.kv_heads;
-    p.tile_rows = int32_t(mma ? MmaShape::rows : SimtShape::rows);
+    int64_t most_rows = 0;
+    for (const PrefixGroup &g : p.groups) most_rows = std::max(most_rows, int64_t(g.members.size()) * p.group);
+    p.tile_rows = int32_t(mma ? MmaShape::rows : most_rows > 32 ? 64 : 16);
+    const int64_t simt_ctas_per_sm = p.tile_rows == 16 ? 4 : 2;
     p.item_words = mma ? 16 : 8;
-    const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtShape::step_tokens) / L.page_size;
+    const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size;
     const auto tiles_of = [&](const PrefixGroup &g) {
         return (int64_t(g.members.size()) * p.group + p.tile_rows - 1) / p.tile_rows;
     };
@@ -160,17 +163,22 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
             pairs += L.kv_heads * ((tiles_of(g) + 1) / 2);
             tiles += L.kv_heads * tiles_of(g);
         }
-        const auto items = [&](int64_t steps) {
+        int64_t values = 0;     // of the partials
+        const auto items = [&](int64_t steps) {     // CTAs of so many steps
             int64_t n = 0;
+            values = 0;
             for (const PrefixGroup &g : p.groups) {
-                const int64_t t = tiles_of(g), s = steps_of(g);
-                n += L.kv_heads * (t / 2 * ((s + steps - 1) / steps) + t % 2 * ((s + 2 * steps - 1) / (2 * steps)));
+                const int64_t t = tiles_of(g), s = steps_of(g), pieces = (s + steps - 1) / steps;
+                n += L.kv_heads * (t / 2 * pieces + t % 2 * ((pieces + 1) / 2));
+                values += L.query_heads * int64_t(g.members.size()) * D * pieces;
             }
             return n;
         };
         const auto waves = [&](int64_t ctas) { return (ctas + sm_count - 1) / sm_count; };
         for (int64_t steps = 1; steps <= most; ++steps) {
-            const int64_t cost = waves(items(steps)) * (MmaShape::overhead_steps + steps) + MmaShape::merge_steps;
+            const int64_t n = items(steps);
+            const int64_t cost = waves(n) * (MmaShape::overhead_steps + steps) + MmaShape::merge_steps +
+                                 values / MmaShape::values_per_step;
             if (cost < best) best = cost, item_steps = steps;
         }
         const int64_t by_pair = waves(pairs) * (MmaShape::overhead_steps + most);
@@ -183,7 +191,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     } else {
         int64_t work = 0;
         for (const PrefixGroup &g : p.groups) work += L.kv_heads * tiles_of(g) * steps_of(g);
-        item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, SimtShape::ctas_per_sm * sm_count));
+        item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, simt_ctas_per_sm * sm_count));
     }
     p.seqs.assign(size_t(L.batch) * 8, 0);
     for (int b = 0; b < L.batch; ++b) p.seqs[size_t(b) * 8] = -1;

@@ -23,109 +23,171 @@
 namespace pd {
 namespace {
 
-constexpr int kSimtRows = 16, kSimtTokens = 32, kSimtThreads = 128;
+constexpr int kSimtThreads = 128, kSimtTokens = 32;
 
-// Four elements as FP32, past L1: another kernel may have written them since this SM last read them.
-template <typename Elt>
-__device__ __forceinline__ float4 load4(const Elt *p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float *p) {
-    return __ldcg(reinterpret_cast<const float4 *>(p));
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
-// One CTA per work item: 16 query rows of one KV head against a piece of the
-// prefix, 32 tokens a step.  Eight threads per row: each scores every eighth
-// token, then adds up its eighth of the head's dims.
-template <typename Elt, int D>
+
+// Shared memory of the FP32 kernel, in floats: queries [R][D + 4], two stages of
+// K [32][D + 4] and V [32][D], weights [R][36], rescale factors [R].  (Row strides
+// 4 floats over a multiple of 32: the rows a warp reads side by side lie 4 banks apart.)
+template <int R, int D>
+struct SimtShape {
+    static constexpr int QS = D + 4, KS = D + 4, PS = kSimtTokens + 4;
+    static constexpr int Q = 0, K = Q + R * QS, V = K + 2 * kSimtTokens * KS, P = V + 2 * kSimtTokens * D,
+                         F = P + R * PS, FLOATS = F + R;
+};
+
+// FP32 prefix kernel: one CTA per work item, R query rows of one KV head against
+// a piece of the prefix, 32 tokens a step, the next step's K and V on their way
+// (cp.async).  CUDA cores, two FMAs to an instruction: the scores in R/16 x 4
+// blocks per thread, the output in R/8 x D/16 ones, so that an operand read from
+// shared memory serves several products.  The online softmax of a row is shared
+// by the eight threads that hold its scores.  Rows of sequences that end inside
+// their prefix (dynamic launches) are dropped by the merge kernel, so only the
+// piece's end needs a mask.
+template <int R, int D>
 __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixArgs a) {
-    constexpr int R = kSimtRows, N = kSimtTokens, KS = D + 4;   // KS: K row stride, rows 4 banks apart
-    __shared__ __align__(16) float qs[R * D], ks[N * KS], vs[N * D], ps[R * N];
+    using S = SimtShape<R, D>;
+    constexpr int N = kSimtTokens, TR = R / 16, OR = R / 8, OD = D / 16;   // rows and dims of a thread's blocks
+    extern __shared__ __align__(16) float sm[];
     // With a suffix decode in front, q, the caches and the lengths are complete (it waited for
     // their writers before any of this grid's CTAs could start) and only its rows are not.
     if (!a.rows) asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 i0 = a.items[2 * blockIdx.x], i1 = a.items[2 * blockIdx.x + 1];
-    const int T = a.page_size, tid = threadIdx.x, r = tid >> 3, c = tid & 7;
-    const int row = i0.w * R + r;                               // row of the group's matrix
-    const int member = row / a.group;
-    const bool on = member < i0.y;
-    const int b = on ? a.members[i0.x + member] : 0;
-    const int head = i0.z * a.group + row % a.group;
-    const int limit = on ? __ldcg(a.lengths + b) : 0;                  // live tokens of the row's sequence
-    const Elt *q = static_cast<const Elt *>(a.q) + (int64_t(b) * a.Hq + head) * D;
-    for (int d = 4 * c; d < D; d += 32) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (on) x = load4<Elt>(q + d);
-        *reinterpret_cast<float4 *>(qs + r * D + d) = x;
+    const int T = a.page_size, tid = threadIdx.x, end = i1.z * T;
+    const uint32_t base = smem_u32(sm);
+    for (int e = tid; e < R * (D / 4); e += kSimtThreads) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4, row = i0.w * R + r, member = row / a.group;
+        const bool on = member < i0.y;
+        const int64_t b = on ? __ldg(a.members + i0.x + member) : 0;
+        copy16(base + (S::Q + r * S::QS + d) * 4,
+               static_cast<const float *>(a.q) + (b * a.Hq + i0.z * a.group + row % a.group) * D + d, on);
     }
-    float m = -INFINITY, l = 0.f, o[D / 8];
-#pragma unroll
-    for (int d = 0; d < D / 8; ++d) o[d] = 0.f;
-    for (int t0 = i1.y * T; t0 < i1.z * T; t0 += N) {
-        __syncthreads();
+    const auto load = [&](int t0, int stage) {
         for (int e = tid; e < N * (D / 4); e += kSimtThreads) {
             const int n = e / (D / 4), d = e % (D / 4) * 4, t = t0 + n;
-            float4 kx = make_float4(0.f, 0.f, 0.f, 0.f), vx = kx;
-            if (t < i1.z * T) {
-                const int64_t at = ((int64_t(a.pages[i1.x + t / T]) * T + t % T) * a.Hkv + i0.z) * D + d;
-                kx = load4<Elt>(static_cast<const Elt *>(a.k) + at);
-                vx = load4<Elt>(static_cast<const Elt *>(a.v) + at);
-            }
-            *reinterpret_cast<float4 *>(ks + n * KS + d) = kx;
-            *reinterpret_cast<float4 *>(vs + n * D + d) = vx;
+            const bool on = t < end;
+            const int64_t page = on ? __ldg(a.pages + i1.x + t / T) : 0;
+            const int64_t at = ((page * T + t % T) * a.Hkv + i0.z) * D + d;
+            copy16(base + (S::K + (stage * N + n) * S::KS + d) * 4, static_cast<const float *>(a.k) + at, on);
+            copy16(base + (S::V + (stage * N + n) * D + d) * 4, static_cast<const float *>(a.v) + at, on);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // scores: tokens tg + 8 j of rows rg + 16 i;  output: rows og + 8 i, dims 4 dg + 64 k + [0, 4)
+    const int tg = tid & 7, rg = tid >> 3, dg = tid & 15, og = tid >> 4;
+    float m[TR], l[TR];
+    f32x2 o[OR][OD / 2];
+#pragma unroll
+    for (int i = 0; i < TR; ++i) m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < OR; ++i)
+#pragma unroll
+        for (int k = 0; k < OD / 2; ++k) o[i][k] = 0;
+    load(i1.y * T, 0);
+    for (int t0 = i1.y * T, stage = 0; t0 < end; t0 += N, stage ^= 1) {
+        if (t0 + N < end) {
+            load(t0 + N, stage ^ 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         __syncthreads();
-        const int live = min(limit, i1.z * T) - t0;             // tokens of this step the row sees (<= 0: none)
-        float s[N / 8], top = m;
+        // ---- scores
+        const float *ks = sm + S::K + (stage * N + tg) * S::KS, *qs = sm + S::Q + rg * S::QS;
+        f32x2 acc[TR][4];
 #pragma unroll
-        for (int k = 0; k < N / 8; ++k) {
-            const float *kr = ks + (c + 8 * k) * KS;
-            float x = 0.f;
-#pragma unroll 8
-            for (int d = 0; d < D; d += 4) {
-                const float4 qa = *reinterpret_cast<const float4 *>(qs + r * D + d);
-                const float4 ka = *reinterpret_cast<const float4 *>(kr + d);
-                x = fmaf(qa.x, ka.x, fmaf(qa.y, ka.y, fmaf(qa.z, ka.z, fmaf(qa.w, ka.w, x))));
+        for (int i = 0; i < TR; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0;
+#pragma unroll 4
+        for (int d = 0; d < D; d += 4) {
+            ulonglong2 q[TR], k[4];
+#pragma unroll
+            for (int i = 0; i < TR; ++i) q[i] = *reinterpret_cast<const ulonglong2 *>(qs + 16 * i * S::QS + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const ulonglong2 *>(ks + 8 * j * S::KS + d);
+#pragma unroll
+            for (int i = 0; i < TR; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fma_f32x2(q[i].y, k[j].y, fma_f32x2(q[i].x, k[j].x, acc[i][j]));
+        }
+        // ---- softmax
+#pragma unroll
+        for (int i = 0; i < TR; ++i) {
+            float s[4], top = m[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 x = unpack_f32x2(acc[i][j]);
+                s[j] = t0 + tg + 8 * j < end ? (x.x + x.y) * a.scale_log2 : -INFINITY;
+                top = fmaxf(top, s[j]);
             }
-            s[k] = c + 8 * k < live ? x * a.scale_log2 : -INFINITY;
-            top = fmaxf(top, s[k]);
+#pragma unroll
+            for (int x = 4; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x));
+            const float ref = top == -INFINITY ? 0.f : top;
+            const float shrink = exp2f(m[i] - ref);
+            m[i] = top;
+            l[i] *= shrink;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(s[j] - ref);
+                l[i] += p;
+                sm[S::P + (rg + 16 * i) * S::PS + tg + 8 * j] = p;
+            }
+            if (tg == 0) sm[S::F + rg + 16 * i] = shrink;
         }
+        __syncthreads();
+        // ---- output
+        const float *vs = sm + S::V + stage * N * D + 4 * dg;
 #pragma unroll
-        for (int x = 4; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, x));
-        const float base = top == -INFINITY ? 0.f : top;        // a row that sees nothing yet
-        const float shrink = exp2f(m - base);
-        l *= shrink;
+        for (int i = 0; i < OR; ++i) {
+            const float f = sm[S::F + og + 8 * i];
+            if (f != 1.f)
 #pragma unroll
-        for (int k = 0; k < N / 8; ++k) {
-            const float p = exp2f(s[k] - base);
-            l += p;
-            ps[r * N + c + 8 * k] = p;
+                for (int k = 0; k < OD / 2; ++k) o[i][k] = mul_f32x2(o[i][k], pack_f32x2(f, f));
         }
-        m = top;
+#pragma unroll 2
+        for (int n = 0; n < N; n += 4) {
+            float4 p[OR];
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) o[d] *= shrink;
-        __syncwarp();
-        const int seen = min(live, N);                          // rows past it may hold anything, NaN too
-        for (int n = 0; n < seen; ++n) {
-            const float p = ps[r * N + n];
+            for (int i = 0; i < OR; ++i) p[i] = *reinterpret_cast<const float4 *>(sm + S::P + (og + 8 * i) * S::PS + n);
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                const float4 x = *reinterpret_cast<const float4 *>(vs + n * D + 32 * d + 4 * c);
-                o[4 * d] = fmaf(p, x.x, o[4 * d]);
-                o[4 * d + 1] = fmaf(p, x.y, o[4 * d + 1]);
-                o[4 * d + 2] = fmaf(p, x.z, o[4 * d + 2]);
-                o[4 * d + 3] = fmaf(p, x.w, o[4 * d + 3]);
+            for (int u = 0; u < 4; ++u) {
+                ulonglong2 v[OD / 4];
+#pragma unroll
+                for (int k = 0; k < OD / 4; ++k) v[k] = *reinterpret_cast<const ulonglong2 *>(vs + (n + u) * D + 64 * k);
+#pragma unroll
+                for (int i = 0; i < OR; ++i) {
+                    const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+                    const f32x2 w2 = pack_f32x2(w, w);
+#pragma unroll
+                    for (int k = 0; k < OD / 4; ++k) {
+                        o[i][2 * k] = fma_f32x2(w2, v[k].x, o[i][2 * k]);
+                        o[i][2 * k + 1] = fma_f32x2(w2, v[k].y, o[i][2 * k + 1]);
+                    }
+                }
             }
         }
+        __syncthreads();        // the stage, the weights and the factors may be overwritten
     }
 #pragma unroll
-    for (int x = 4; x > 0; x >>= 1) l += __shfl_xor_sync(kFullMask, l, x);
-    if (on) {
-        float *po = a.part_o + int64_t(i1.w) * R * D + r * 8 + c % 2 * 4;
+    for (int i = 0; i < TR; ++i) {
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-            *reinterpret_cast<float4 *>(po + (4 * d + c / 2) * (R * 8)) =
-                make_float4(o[4 * d], o[4 * d + 1], o[4 * d + 2], o[4 * d + 3]);
-        if (c == 0) a.part_ml[int64_t(i1.w) * R + r] = make_float2(m, l);
+        for (int x = 4; x > 0; x >>= 1) l[i] += __shfl_xor_sync(kFullMask, l[i], x);
+        if (tg == 0) a.part_ml[int64_t(i1.w) * R + rg + 16 * i] = make_float2(m[i], l[i]);
     }
+    float *po = a.part_o + int64_t(i1.w) * R * D;
+#pragma unroll
+    for (int i = 0; i < OR; ++i)
+#pragma unroll
+        for (int k = 0; k < OD / 4; ++k) {
+            const int d = 4 * dg + 64 * k;
+            *reinterpret_cast<ulonglong2 *>(po + (d / 8 * R + og + 8 * i) * 8 + d % 8) =
+                make_ulonglong2(o[i][2 * k], o[i][2 * k + 1]);
+        }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // the suffix decode's rows are complete when this grid is
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
@@ -159,7 +221,7 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const Prefi
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // a dynamic launch's sequence that ends inside its prefix
-    if (sizeof(Elt) == 2 && prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size) {
+    if (prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size) {
         if (way == 0) row_inside<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, b, lane);
         pieces = 0;
         on = false;
@@ -237,6 +299,31 @@ MmaEntry mma_entry_for(const pd_layout &L) {
     return L.page_size == 16 ? mma_entry<128, 16>() : mma_entry<128, 32>();
 }
 
+using SimtKernel = void (*)(const PrefixArgs);
+struct SimtEntry {
+    SimtKernel kernel;
+    size_t smem;
+};
+template <int D>
+SimtEntry simt_entry(int rows) {
+    if (rows == 16) return {prefix_simt_kernel<16, D>, SimtShape<16, D>::FLOATS * 4};
+    return {prefix_simt_kernel<64, D>, SimtShape<64, D>::FLOATS * 4};
+}
+
+// Allow the prefix kernel of this plan its shared memory.
+cudaError_t allow_smem(const pd_prefix_plan &p) {
+    const void *kernel;
+    size_t smem;
+    if (p.dtype == PD_FLOAT16) {
+        const MmaEntry e = mma_entry_for(p.layout);
+        kernel = reinterpret_cast<const void *>(e.kernel), smem = e.smem;
+    } else {
+        const SimtEntry e = p.layout.head_dim == 64 ? simt_entry<64>(p.tile_rows) : simt_entry<128>(p.tile_rows);
+        kernel = reinterpret_cast<const void *>(e.kernel), smem = e.smem;
+    }
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+}
+
 template <int D>
 cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CUtensorMap &map_k,
                           const CUtensorMap &map_v, cudaStream_t stream) {
@@ -247,7 +334,8 @@ cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CU
         err = launch_dependent(e.kernel, items, e.threads, e.smem, stream, map_k, map_v, a);
         if (p.direct) return err;
     } else if (items) {
-        err = launch_dependent(prefix_simt_kernel<float, D>, items, kSimtThreads, 0, stream, a);
+        const SimtEntry e = simt_entry<D>(p.tile_rows);
+        err = launch_dependent(e.kernel, items, kSimtThreads, e.smem, stream, a);
     }
     if (err != cudaSuccess) return err;
     const int64_t rows = int64_t(a.B) * a.Hq, per_cta = kMergeThreads / (D / 8) / p.merge_ways;
@@ -426,11 +514,7 @@ PD_API pd_status pd_prefix_plan_bind(pd_prefix_plan *p, void *buffer, size_t byt
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
     cudaError_t err = prev == p->device ? cudaSuccess : cudaSetDevice(p->device);
     const auto st = static_cast<cudaStream_t>(stream);
-    if (err == cudaSuccess && p->dtype == PD_FLOAT16) {
-        const MmaEntry e = mma_entry_for(p->layout);
-        err = cudaFuncSetAttribute(reinterpret_cast<const void *>(e.kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   int(e.smem));
-    }
+    if (err == cudaSuccess) err = allow_smem(*p);
     if (err == cudaSuccess)
         err = cudaMemcpyAsync(dev, p->host_image.data(), p->host_image.size(), cudaMemcpyHostToDevice, st);
     if (err == cudaSuccess) err = cudaStreamSynchronize(st);

@@ -7,15 +7,15 @@
 //   * split: one row tile whose pages are cut in two runs; each stream loads
 //     its own steps (few rows: the prefix's bytes bound the kernel, and two
 //     streams keep both the loads and the softmax busy).
-// Roles (11 warps):
+// Roles (12 warps):
 //   * warps 0-3 / 4-7: softmax of stream 0 / 1, one thread per query row
 //     (tensor-memory lane).  S is read from tensor memory, the weights go back
 //     as FP16 over the scores' own columns, where the PV product reads them as
 //     its A operand;
-//   * warp 8, one elected lane: TMA loads of K and V steps into one ring, one box
-//     per page;
-//   * warps 9 / 10, one elected lane each: the MMAs of stream 0 / 1.  S = Q K^T
-//     (M 128, N 64), O += P V (M 128, N = head dim).
+//   * warps 8 / 9, one elected lane each: the MMAs of stream 0 / 1.  S = Q K^T
+//     (M 128, N 64), O += P V (M 128, N = head dim);
+//   * warps 10 / 11, one elected lane each: TMA loads of K and V steps into rings
+//     of shared memory, one box per page.
 // Each stream has two score blocks, so that a softmax finds its next scores
 // ready: those of step i + 2 are issued once the PV product of step i, whose
 // weights lie in the same block, has completed.  (Steps of 128 tokens leave
@@ -61,8 +61,8 @@ struct PrefixShape {
     static constexpr int Q_BYTES = NBOX * Q_BOX;
     static constexpr int K_SLOTS = D == 128 ? 2 : 4, V_SLOTS = D == 128 ? 3 : 4;   // of one step, per stream
     static constexpr int SLOTS = 2 * (K_SLOTS + V_SLOTS);
-    static constexpr int SOFTMAX_WARPS = 8, W_LOAD = 8, W_MMA = 9;
-    static constexpr int THREADS = 352;                 // W_MMA + t issues stream t's MMAs
+    static constexpr int SOFTMAX_WARPS = 8, W_MMA = 8, W_LOAD = 10;     // and one more of each kind
+    static constexpr int THREADS = 384;
     // tensor memory: score blocks (weights in their first half) [stream][2], outputs [stream]
     static constexpr int S_COL = 0, O_COL = 4 * NS;
     static constexpr int TMEM_COLS = 512;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     const PrefixItem it = prefix_item(a, blockIdx.x);
     const int n0 = it.s0.steps(NP), n1 = it.s1.steps(NP);   // n1 <= n0; paired: n1 == n0
     const bool paired = it.kind == kItemPaired;
-    // Warps 8 to 10 stay converged, and what they hand to the hardware is the same in all lanes
+    // Warps 8 to 11 stay converged, and what they hand to the hardware is the same in all lanes
     // (reductions over the warp give the compiler the proof): operands then live in uniform registers.
     const auto uniform = [](int x) { return __reduce_max_sync(kFullMask, x); };
     if (it.kind == kItemCopy) {
@@ -226,26 +226,26 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         *abort_flag = 1;
     };
 
-    if (warp == S::W_LOAD) {
+    if (warp >= S::W_LOAD) {
         // ------------------------------------------------------------ loads
+        const int w = warp - S::W_LOAD;
         const bool upaired = uniform(it.kind) == kItemPaired;
-        const int un0 = uniform(n0), un1 = upaired ? 0 : uniform(n1);
-        const int first0 = uniform(it.s0.first), end0 = uniform(it.s0.end);
-        const int first1 = uniform(it.s1.first), end1 = uniform(it.s1.end);
         const int head = uniform(it.head);
-        // one of the four sequences of steps: K or V of a stream, with page ids 32 at a time, one per lane
+        // one sequence of steps: K or V of a stream, with page ids 32 at a time, one per lane
         struct Feed {
             RingCursor at;
-            int window = 0, base = -64, steps = 0;
+            int first, end, steps, done, window, base;
         };
-        Feed k0{k_cursor<S>(0, upaired)}, k1{k_cursor<S>(1, upaired)}, v0{v_cursor<S>(0, upaired)},
-            v1{v_cursor<S>(1, upaired)};
+        const auto feed = [&](RingCursor at, const PrefixStream &st) {
+            return Feed{at, uniform(st.first), uniform(st.end), uniform(st.steps(NP)), 0, 0, -64};
+        };
         bool ok = true;
-        const auto load = [&](Feed &f, int first, int end, bool is_v) {
-            const int p0 = first + f.steps * NP, n = min(NP, end - p0);
+        const auto load = [&](Feed &f, bool is_v) {
+            if (!ok || f.done >= f.steps) return;
+            const int p0 = f.first + f.done * NP, n = min(NP, f.end - p0);
             if (p0 + NP > f.base + 32) {
                 f.base = p0;
-                f.window = p0 + lane < end ? __ldg(a.pages + it.page0 + p0 + lane) : 0;
+                f.window = p0 + lane < f.end ? __ldg(a.pages + it.page0 + p0 + lane) : 0;
             }
             // (a fresh barrier's preceding phase counts as complete: the first pass does not wait)
             ok = __all_sync(kFullMask, mbar_wait(smem_u32(empty + f.at.slot), uint32_t(f.at.phase ^ 1))) &&
@@ -263,28 +263,30 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 else tma_load_5d_warp(dst + p * S::PAGE_BYTES, &tm_k, 0, 0, head * S::NBOX, 0, id, bar);
             }
             f.at.next();
-            ++f.steps;
+            ++f.done;
         };
-        // K steps 0 and 1, then V step i and K step i + 2
-        for (int j = -2; j < un0 && ok; ++j) {
-            if (j >= 0) load(v0, first0, end0, true);
-            if (ok && j >= 0 && j < un1) load(v1, first1, end1, true);
-            if (ok && j + 2 < un0) load(k0, first0, end0, false);
-            if (ok && j + 2 < un1) load(k1, first1, end1, false);
+        // paired streams: one warp brings K, the other V; split streams: a warp each, K two steps ahead
+        Feed fk = feed(k_cursor<S>(upaired ? 0 : w, upaired), it.s(upaired ? 0 : w));
+        Feed fv = feed(v_cursor<S>(upaired ? 0 : w, upaired), it.s(upaired ? 0 : w));
+        if (upaired && w == 0) fv.steps = 0;
+        if (upaired && w == 1) fk.steps = 0;
+        load(fk, false);
+        load(fk, false);
+        while (ok && (fk.done < fk.steps || fv.done < fv.steps)) {
+            load(fv, true);
+            load(fk, false);
         }
         if (!ok && lane == 0) fail_wait();
         // no copy is in flight when the CTA ends, whatever became of its readers
         const auto drain = [&](const Feed &f) {
-            for (int i = 0; i < min(f.at.count, f.steps); ++i) {
+            for (int i = 0; i < min(f.at.count, f.done); ++i) {
                 const int slot = f.at.first + i;
                 const int phase = slot < f.at.slot ? f.at.phase : f.at.phase ^ 1;    // of its last use
                 if (!mbar_wait(smem_u32(full + slot), uint32_t(phase)) && lane == 0) fail_wait();
             }
         };
-        drain(k0);
-        drain(k1);
-        drain(v0);
-        drain(v1);
+        drain(fk);
+        drain(fv);
         __syncwarp();
     } else if (warp >= S::W_MMA) {
         // ------------------------------------------------------------ MMAs of one stream (one elected lane)

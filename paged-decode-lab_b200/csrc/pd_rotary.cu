@@ -89,7 +89,6 @@ __device__ __forceinline__ void store_piece(Elt *p, const Piece<Elt> &r) {
 }
 
 // A piece in FP32, two elements to a register pair, and back (one rounding).
-using f32x2 = unsigned long long;
 __device__ __forceinline__ void widen(f32x2 (&x)[2], const Piece<__half> &p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
