@@ -401,6 +401,8 @@ typedef struct pd_prefix_info {
     int32_t members;             /* sequences in a group */
     int32_t tile_rows;           /* query rows of one prefix tile */
     int32_t items;               /* CTAs of the prefix kernel */
+    int32_t item_words;          /* int32 words of one work item (pd_prefix_plan_copy_items) */
+    int32_t direct;              /* 1: the prefix kernel writes the output, 0: partials and a merge kernel */
     int32_t suffix_launch;       /* 1: the decode kernel runs (some sequence goes on behind its prefix) */
     int32_t dynamic;
     int64_t shared_pages;        /* page reads saved: sum over groups of (members - 1) * pages */
@@ -410,8 +412,9 @@ typedef struct pd_prefix_info {
 /* Build a plan from host metadata (see pd_plan_create; copied).  Groups: group
  * g has members[indptr[g]] .. members[indptr[g + 1] - 1] (sequences, each in
  * at most one group) sharing their first pages[g] pages, all of them whole
- * (lengths >= pages * page_size) and equal in the table.  group_count < 0
- * finds the groups in the table: leading pages that are worth sharing.
+ * (lengths >= pages * page_size) and equal in the table.  group_count -2 finds
+ * the groups in the table, -1 uses the found ones only if they save enough
+ * (otherwise none).
  * max_lengths (NULL: a static plan) as in pd_plan_create_dynamic.  device < 0
  * builds a host-only plan. */
 pd_status pd_prefix_plan_create(const pd_layout *layout, const int32_t *table, int64_t table_width,
@@ -424,6 +427,14 @@ pd_status pd_prefix_plan_get_info(const pd_prefix_plan *plan, pd_prefix_info *in
 /* The plan's groups: group[b] the group of sequence b or -1 (int32 [batch]),
  * pages[g] its shared pages (int32 [groups]).  Either may be NULL. */
 pd_status pd_prefix_plan_copy_groups(const pd_prefix_plan *plan, int32_t *group, int32_t *pages);
+
+/* The prefix kernel's work items, for inspection and tests (info.items *
+ * info.item_words int32).  FP32 (8 words): first member, members, KV head, row
+ * tile, first of the group's pages, first page, end page, partial slot.  FP16
+ * (16): first member, members, KV head, kind (0 two runs of pages of one tile, 1
+ * two tiles over one run, 2 copy these sequences' rows), first of the group's
+ * pages, shared pages, 0, 0, and twice: row tile, first page, end page, slot. */
+pd_status pd_prefix_plan_copy_items(const pd_prefix_plan *plan, int32_t *items);
 
 /* As pd_plan_device_bytes / pd_plan_bind. */
 size_t pd_prefix_plan_device_bytes(const pd_prefix_plan *plan);

@@ -17,7 +17,7 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 }  // namespace
 
 void find_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,
-                        int64_t overhead_pages, std::vector<PrefixGroup> &groups) {
+                        std::vector<PrefixGroup> &groups) {
     groups.clear();
     const int B = layout.batch;
     const auto full = [&](int b) { return int64_t(lengths[b]) / layout.page_size; };   // whole live pages
@@ -59,7 +59,7 @@ void find_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t w
                 r.inside.push_back(closed);
                 r.saved += runs[closed].saved;
             }
-            const int64_t own = int64_t(r.right - r.left) * r.pages - overhead_pages;
+            const int64_t own = int64_t(r.right - r.left) * r.pages;
             r.whole = own >= r.saved && own > 0;
             if (r.whole) r.saved = own;
             left = r.left;
@@ -117,7 +117,8 @@ pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int
 
 namespace {
 
-// FP32 (CUDA cores): tiles of 16 rows, or of 64 where a group has more than 32,
+// FP32 (CUDA cores): tiles of 16 rows, or of 64 where a group has more than 16
+// (32 rows: half a tile of 64 runs at 13 TFLOP/s, two of 16 at 10),
 // 32-token steps, about as many CTAs as are resident at once.
 struct SimtPlan {
     static constexpr int64_t step_tokens = 32;
@@ -141,7 +142,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     p.group = L.query_heads / L.kv_heads;
     int64_t most_rows = 0;
     for (const PrefixGroup &g : p.groups) most_rows = std::max(most_rows, int64_t(g.members.size()) * p.group);
-    p.tile_rows = int32_t(mma ? MmaShape::rows : most_rows > 32 ? 64 : 16);
+    p.tile_rows = int32_t(mma ? MmaShape::rows : most_rows > 16 ? 64 : 16);
     const int64_t simt_ctas_per_sm = p.tile_rows == 16 ? 4 : 2;
     p.item_words = mma ? 16 : 8;
     const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size;

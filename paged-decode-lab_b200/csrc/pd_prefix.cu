@@ -6,6 +6,7 @@
 // o = sum 2^(s - m) v  (base 2: scores carry log2(e)).  The tokens behind the
 // prefix go through the decode kernel, which gives (m', l', o'), and
 // out = (2^(m-M) o + 2^(m'-M) l' o') / (2^(m-M) l + 2^(m'-M) l'),  M = max(m, m').
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -384,6 +385,12 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.P = p->layout.physical_pages;
     a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(p->layout.head_dim)));
     pd_status s = PD_OK;
+    if (p->items.empty() && dtype == PD_FLOAT32) {      // nothing shared, nothing to convert
+        s = table ? pd_decode_dynamic(p->suffix, q, k, v, dtype, table, lengths, static_cast<float *>(out), nullptr, stream)
+                  : pd_decode(p->suffix, q, k, v, dtype, static_cast<float *>(out), stream);
+        if (prev >= 0 && prev != p->device) cudaSetDevice(prev);
+        return s;
+    }
     alignas(64) CUtensorMap map_k, map_v;
     if (dtype == PD_FLOAT16 && !p->items.empty()) s = encode_prefix_maps(*p->suffix, k, v, &map_k, &map_v);
     if (s == PD_OK && !p->suffix_empty) {
@@ -404,6 +411,13 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     return s;
 }
 
+// Found groups are used where they save reading this much again.  The decode
+// kernel reads a shared page's copies from L2 at about 13 TB/s, and the prefix and merge
+// kernels cost about 20 us.  Measured, us shared / not: 32 sequences of 32:8 FP16 heads behind 1024,
+// 2048 and 4096 tokens (130, 260 and 520 MB) 30 / 24, 32 / 34, 36 / 53; 64 of 32:1 behind 2048
+// and 8192 (66, 264 MB) 32 / 19, 44 / 46; 16 of 32:8 FP32 behind 2048 and 4096 (252, 503 MB) 51 / 49, 71 / 85.
+constexpr int64_t kWorthBytes = int64_t(256) << 20;
+
 pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t width, const int32_t *lengths,
                       const int32_t *max_lengths, int32_t group_count, const int32_t *indptr, const int32_t *members,
                       const int32_t *pages, pd_dtype dtype, int32_t device, pd_prefix_plan &p) {
@@ -418,7 +432,12 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t wid
     p.width = width;
     p.dynamic = max_lengths != nullptr;
     if (group_count < 0) {
-        find_prefix_groups(p.layout, table, width, lengths, 0, p.groups);
+        find_prefix_groups(p.layout, table, width, lengths, p.groups);
+        int64_t saved = 0;
+        for (const PrefixGroup &g : p.groups) saved += int64_t(g.members.size() - 1) * g.pages;
+        const int64_t page_bytes = 2 * int64_t(layout->page_size) * layout->kv_heads * layout->head_dim *
+                                   (dtype == PD_FLOAT16 ? 2 : 4);
+        if (group_count == -1 && saved * page_bytes < kWorthBytes) p.groups.clear();
     } else {
         if (group_count > 0 && (!indptr || !members || !pages))
             return fail(PD_ERR_VALUE, "group arrays must not be NULL");
@@ -481,6 +500,8 @@ PD_API pd_status pd_prefix_plan_get_info(const pd_prefix_plan *p, pd_prefix_info
     }
     info->tile_rows = p->tile_rows;
     info->items = int32_t(p->items.size() / p->item_words);
+    info->item_words = p->item_words;
+    info->direct = p->direct ? 1 : 0;
     info->suffix_launch = p->suffix_empty ? 0 : 1;
     info->dynamic = p->dynamic ? 1 : 0;
     info->device_bytes = int64_t(p->image.bytes);
@@ -496,6 +517,12 @@ PD_API pd_status pd_prefix_plan_copy_groups(const pd_prefix_plan *p, int32_t *gr
         if (group)
             for (const int32_t b : p->groups[g].members) group[b] = int32_t(g);
     }
+    return PD_OK;
+}
+
+PD_API pd_status pd_prefix_plan_copy_items(const pd_prefix_plan *p, int32_t *items) {
+    if (!p || !items) return fail(PD_ERR_VALUE, "plan and items must not be NULL");
+    std::copy(p->items.begin(), p->items.end(), items);
     return PD_OK;
 }
 

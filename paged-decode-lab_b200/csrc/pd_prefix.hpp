@@ -55,9 +55,9 @@ namespace pd {
 
 // Groups of sequences whose leading pages are the same.  A candidate is all
 // sequences that start with some pages; disjoint candidates are chosen so that
-// the page reads saved, less `overhead_pages` per group, are the most.
+// the page reads saved are the most.
 void find_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,
-                        int64_t overhead_pages, std::vector<PrefixGroup> &groups);
+                        std::vector<PrefixGroup> &groups);
 
 // Check the groups against the table and lengths.
 pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,

@@ -42,7 +42,8 @@ class PlanInfo(ctypes.Structure):
 
 class PrefixInfo(ctypes.Structure):
     _fields_ = [("groups", ctypes.c_int32), ("members", ctypes.c_int32), ("tile_rows", ctypes.c_int32),
-                ("items", ctypes.c_int32), ("suffix_launch", ctypes.c_int32), ("dynamic", ctypes.c_int32),
+                ("items", ctypes.c_int32), ("item_words", ctypes.c_int32), ("direct", ctypes.c_int32),
+                ("suffix_launch", ctypes.c_int32), ("dynamic", ctypes.c_int32),
                 ("shared_pages", ctypes.c_int64), ("device_bytes", ctypes.c_int64)]
 
 
@@ -99,6 +100,7 @@ SIGNATURES = {
     "pd_prefix_plan_destroy": (None, [_vp]),
     "pd_prefix_plan_get_info": (_c_int32, [_vp, ctypes.POINTER(PrefixInfo)]),
     "pd_prefix_plan_copy_groups": (_c_int32, [_vp, _vp, _vp]),
+    "pd_prefix_plan_copy_items": (_c_int32, [_vp, _vp]),
     "pd_prefix_plan_device_bytes": (_c_size, [_vp]),
     "pd_prefix_plan_bind": (_c_int32, [_vp, _vp, _c_size, _vp]),
     "pd_prefix_decode": (_c_int32, [_vp, _vp, _vp, _vp, _c_int32, _vp, _vp]),

@@ -17,10 +17,10 @@ from .layout import Layout, validate_metadata
 from .rotary import _cuda_device, _dtype_code, _int32
 from .runtime import _check_limits
 
-__all__ = ["SharedPrefixPlan", "find_prefixes"]
+__all__ = ["SharedPrefixPlan", "find_prefixes", "inspect_prefix_plan"]
 
 
-def _native_plan(layout, table, lengths, prefixes, max_lengths, code, device_index):
+def _native_plan(layout, table, lengths, prefixes, max_lengths, code, device_index, find=-1):
     lib = _native.load()
     c_layout = _native.Layout(layout.batch, layout.query_heads, layout.kv_heads, layout.head_dim,
                               layout.page_size, layout.physical_pages)
@@ -28,7 +28,7 @@ def _native_plan(layout, table, lengths, prefixes, max_lengths, code, device_ind
     lengths = np.ascontiguousarray(lengths, dtype=np.int32)
     if max_lengths is not None:
         max_lengths = np.ascontiguousarray(max_lengths, dtype=np.int32)
-    count, arrays = -1, [None, None, None]
+    count, arrays = find, [None, None, None]
     if prefixes is not None:
         members = [np.asarray(m) for m, _ in prefixes]
         if any(m.ndim != 1 or (m.size and m.dtype.kind not in "iu") for m in members):
@@ -61,16 +61,37 @@ def _groups(lib, handle, batch):
 
 
 def find_prefixes(layout: Layout, table, lengths, *, dtype="float16"):
-    """The prefix groups a plan finds by itself, [(sequence indices, pages)] (no GPU needed)."""
+    """The groups of sequences that start with the same pages, [(sequence indices, pages)].
+
+    Each group is all sequences with some leading pages in common, chosen so that the page reads
+    that sharing saves are the most.  No GPU needed; a plan uses them by itself only where they
+    save enough.
+    """
     _check_limits(layout, 256, "serial")
     table, lengths = validate_metadata(layout, table, lengths)
     lib = _native.load()
     code = {"float16": _native.PD_FLOAT16, "float32": _native.PD_FLOAT32}[dtype]
-    handle = _native_plan(layout, table, lengths, None, None, code, -1)
+    handle = _native_plan(layout, table, lengths, None, None, code, -1, find=-2)
     try:
         return _groups(lib, handle, layout.batch)[1]
     finally:
         lib.pd_prefix_plan_destroy(handle)
+
+
+def inspect_prefix_plan(layout: Layout, table, lengths, *, prefixes=None, dtype="float16", max_lengths=None):
+    """A host-only plan's (info, groups, work items) as pd_prefix_plan_copy_items lays them out (no GPU needed)."""
+    _check_limits(layout, 256, "serial")
+    table, lengths = validate_metadata(layout, table, lengths)
+    lib = _native.load()
+    code = {"float16": _native.PD_FLOAT16, "float32": _native.PD_FLOAT32}[dtype]
+    handle = _native_plan(layout, table, lengths, prefixes, max_lengths, code, -1)
+    try:
+        info, groups = _groups(lib, handle, layout.batch)
+        items = np.empty((info.items, info.item_words), dtype=np.int32)
+        _native.check(lib.pd_prefix_plan_copy_items(handle, items.ctypes.data))
+    finally:
+        lib.pd_prefix_plan_destroy(handle)
+    return {name: getattr(info, name) for name, _ in info._fields_}, groups, items
 
 
 class SharedPrefixPlan:
@@ -79,8 +100,8 @@ class SharedPrefixPlan:
     ``layout``, ``table`` and ``lengths`` as for ``DecodePlan``.  ``prefixes``
     lists the groups as (sequence indices, pages): each sequence in at most one
     group, whose first ``pages`` pages are the same and whole in all of them;
-    None finds the groups in the table where sharing pays (``find_prefixes``), [] shares
-    nothing.  ``max_lengths`` makes a dynamic plan (``run_dynamic``).  ``run``
+    None takes those of ``find_prefixes`` if they save reading 256 MB or more (below that
+    the decode kernel reads the copies from L2 in less time), [] shares nothing.  ``max_lengths`` makes a dynamic plan (``run_dynamic``).  ``run``
     returns the plan's own [batch, query_heads, head_dim] output in ``dtype``
     (the inputs' type; sums are FP32), which the next run overwrites.  Launch a
     plan from one stream at a time.

@@ -200,6 +200,53 @@ def test_dead_rows_of_a_live_length_inside_the_prefix():
     close(out, *exact(q, k, v, table, live))
 
 
+@pytest.mark.parametrize("members,pages,heads,kv,direct", [
+    (400, 32, 64, 8, 1),      # more row tiles than SMs: a CTA per pair of them, and one odd tile
+    (200, 32, 64, 8, 1),      # a CTA per tile
+    (64, 512, 32, 1, 0),      # pairs of tiles in pieces
+    (40, 700, 8, 2, 0)])      # odd tile counts in pieces
+def test_every_way_to_cut_the_work(members, pages, heads, kv, direct):
+    layout, table, lengths, groups, q, k, v = case([(pages, [i % 40 for i in range(members)])], [7, 0], heads, kv, 128,
+                                                   16, F16)
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=groups)
+    assert plan.info.direct == direct
+    out = plan.run(q, k, v)
+    some = np.r_[0:members + 2:9, members, members + 1]
+    close(out[some], *exact(q[some], k, v, table[some], lengths[some]))
+    first = out.clone()
+    assert all(torch.equal(plan.run(q, k, v), first) for _ in range(5)) and plan.read_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_live_lengths_inside_a_long_prefix(dtype):
+    """As above where the prefix is cut in pieces for the merge kernel."""
+    layout, table, lengths, members, q, k, v = case([(600, [4, 0, 9, 20])], [12, 0], 8, 2, 128, 16, dtype)
+    k[k.isnan()], v[v.isinf()] = 0.25, 0.5
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=members, dtype=dtype, max_lengths=lengths)
+    assert not plan.info.direct
+    live = lengths.copy()
+    a, b, c, _ = members[0][0]
+    live[a], live[b], live[c] = 0, 1, 9000
+    out = plan.run_dynamic(q, k, v, torch.tensor(table, device="cuda"), torch.tensor(live, device="cuda"))
+    close(out, *exact(q, k, v, table, live))
+    assert plan.read_errors() == 0
+
+
+def test_another_stream_and_interleaved_plans():
+    """Two plans of different shapes taking turns on a stream of their own."""
+    sets = [case([(30, [3, 9])], [4], 8, 2, 128, 16, F16, seed=1), case([(12, list(range(40)))], [], 32, 1, 64, 32, F16, seed=2)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        plans = [SharedPrefixPlan(s[0], s[1], s[2], prefixes=s[3]) for s in sets]
+        for _ in range(20):
+            outs = [p.run(*s[4:]) for p, s in zip(plans, sets)]
+    stream.synchronize()
+    for s, out, plan in zip(sets, outs, plans):
+        close(out, *exact(*s[4:], s[1], s[2]))
+        assert plan.read_errors() == 0
+
+
 def test_pages_past_32_bit_offsets():
     page, kv, D = 32, 8, 128
     pages = (1 << 31) // (page * kv * D) + 40

@@ -6,7 +6,7 @@ import pytest
 
 from paged_decode import _native
 from paged_decode.layout import Layout
-from paged_decode.prefix import _native_plan, find_prefixes
+from paged_decode.prefix import _native_plan, find_prefixes, inspect_prefix_plan
 from paged_decode.workload import config2
 
 
@@ -115,3 +115,81 @@ def test_rotary_entry_points_refuse_bad_arguments():
         bad = _native.Layout.from_buffer_copy(layout)
         setattr(bad, field, value)
         assert append(l=bad) == V, field
+
+
+def shared_batch(counts, others, heads, kv, page, D=64):
+    """A table of groups with (members, pages) and other sequences of one page."""
+    rows, lengths, members, pool = [], [], [], 0
+    for n, pages in counts:
+        shared = list(range(pool, pool + pages))
+        pool += pages
+        members.append((list(range(len(rows), len(rows) + n)), pages))
+        for _ in range(n):
+            rows.append(shared)
+            lengths.append(pages * page)
+    for _ in range(others):
+        rows.append([pool])
+        pool += 1
+        lengths.append(3)
+    width = max(map(len, rows))
+    table = np.full((len(rows), width), -1, dtype=np.int32)
+    for b, r in enumerate(rows):
+        table[b, :len(r)] = r
+    return Layout(len(rows), heads, kv, D, page, max(pool, 1)), table, np.array(lengths), members
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+@pytest.mark.parametrize("heads,kv,page", [(32, 8, 16), (32, 1, 32), (40, 8, 32), (64, 2, 16), (6, 6, 32)])
+@pytest.mark.parametrize("counts,others", [([(1, 1)], 0), ([(4, 64)], 3), ([(3, 5), (70, 33), (2, 200)], 1),
+                                           ([(400, 20)], 0), ([(64, 512)], 0), ([(2, 4000)], 5)])
+def test_work_items_cover_every_row_and_page_once(dtype, heads, kv, page, counts, others):
+    layout, table, lengths, members = shared_batch(counts, others, heads, kv, page)
+    info, groups, items = inspect_prefix_plan(layout, table, lengths, prefixes=members, dtype=dtype)
+    assert len(items) == info["items"] and info["members"] == sum(n for n, _ in counts)
+    rows_per_tile, seen, copied, slots = info["tile_rows"], {}, 0, []
+    first_member, first_page = 0, 0
+    starts = {}                                      # the group of a first member
+    for g, (n, pages) in enumerate(counts):
+        starts[first_member] = (g, first_page)
+        first_member, first_page = first_member + n, first_page + pages
+    streams = []                                     # (group, head, tile, first, end, slot)
+    for it in items:
+        it = [int(x) for x in it]
+        if info["item_words"] == 16 and it[3] == 2:
+            assert it[0] >= first_member and 1 <= it[1] <= 4
+            copied += it[1]
+            continue
+        g, page0 = starts[it[0]]
+        assert it[1] == counts[g][0] and it[4] == page0
+        if info["item_words"] == 8:
+            streams.append((g, it[2], it[3], it[5], it[6], it[7]))
+            continue
+        assert it[5] == counts[g][1]
+        a, b = it[8:12], it[12:16]
+        if it[3] == 1:                               # two tiles, one run
+            assert b[0] == a[0] + 1 and a[1:3] == b[1:3]
+        else:                                        # one tile, the longer run first
+            assert a[0] == b[0] and a[2] - a[1] >= b[2] - b[1]
+        streams += [(g, it[2], *x) for x in (a, b) if x[2] > x[1]]
+    for g, head, tile, first, end, slot in streams:
+        assert 0 <= first < end <= counts[g][1] and 0 <= head < kv
+        for p in range(first, end):
+            key = (g, head, tile, p)
+            assert key not in seen
+            seen[key] = 1
+        slots.append(slot)
+    want = sum(kv * -(-n * (heads // kv) // rows_per_tile) * pages for n, pages in counts)
+    assert len(seen) == want
+    if info["direct"]:
+        assert copied == others                      # every row of the batch is written
+    else:
+        assert copied == 0 and sorted(slots) == list(range(len(slots)))
+
+
+def test_sharing_is_left_out_where_it_saves_little():
+    layout, table, lengths, members = shared_batch([(8, 64)], 2, 32, 8, 16, D=128)
+    assert inspect_prefix_plan(layout, table, lengths)[0]["groups"] == 0
+    assert inspect_prefix_plan(layout, table, lengths, prefixes=members)[0]["groups"] == 1
+    layout, table, lengths, members = shared_batch([(64, 256)], 2, 32, 8, 16, D=128)     # 63 * 256 * 64 KiB saved
+    info, groups, _ = inspect_prefix_plan(layout, table, lengths)
+    assert info["groups"] == 1 and groups[0][1] == 256 and info["shared_pages"] == 63 * 256
