@@ -402,7 +402,7 @@ typedef struct pd_prefix_info {
     int32_t tile_rows;           /* query rows of one prefix tile */
     int32_t items;               /* CTAs of the prefix kernel */
     int32_t item_words;          /* int32 words of one work item (pd_prefix_plan_copy_items) */
-    int32_t direct;              /* 1: the prefix kernel writes the output, 0: partials and a merge kernel */
+    int32_t suffix_ctas;         /* SMs that decode the suffixes beside the prefix kernel; 0: behind it, on all */
     int32_t suffix_launch;       /* 1: the decode kernel runs (some sequence goes on behind its prefix) */
     int32_t dynamic;
     int64_t shared_pages;        /* page reads saved: sum over groups of (members - 1) * pages */
@@ -432,8 +432,8 @@ pd_status pd_prefix_plan_copy_groups(const pd_prefix_plan *plan, int32_t *group,
  * info.item_words int32).  FP32 (8 words): first member, members, KV head, row
  * tile, first of the group's pages, first page, end page, partial slot.  FP16
  * (16): first member, members, KV head, kind (0 two runs of pages of one tile, 1
- * two tiles over one run, 2 copy these sequences' rows), first of the group's
- * pages, shared pages, 0, 0, and twice: row tile, first page, end page, slot. */
+ * two tiles over one run), first of the group's pages, 0, 0, 0, and twice: row
+ * tile, first page, end page, slot. */
 pd_status pd_prefix_plan_copy_items(const pd_prefix_plan *plan, int32_t *items);
 
 /* As pd_plan_device_bytes / pd_plan_bind. */

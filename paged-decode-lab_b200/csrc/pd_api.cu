@@ -284,7 +284,7 @@ pd_status launch(pd_plan *p, const void *k, const void *v, pd_dtype dtype, int m
 
 pd_status decode_impl(pd_plan *p, const void *q, const void *k, const void *v, pd_dtype dtype,
                       float *out, float *stats, void *stream, const int32_t *table = nullptr,
-                      const int32_t *lengths = nullptr, const DecodeArgs *exchange = nullptr) {
+                      const int32_t *lengths = nullptr, const DecodeArgs *exchange = nullptr, bool beside = false) {
     pd_status s = check_bound(p);
     if (s != PD_OK) return s;
     if ((s = check_dtype(p, dtype)) != PD_OK) return s;
@@ -299,6 +299,7 @@ pd_status decode_impl(pd_plan *p, const void *q, const void *k, const void *v, p
     DecodeArgs args = make_args(p, q, out, stats);
     if (table) args.table = table;
     if (lengths) args.lengths = lengths;
+    args.beside = beside ? 1 : 0;
     if (exchange) {
         std::copy(exchange->xpeer, exchange->xpeer + kMaxRanks, args.xpeer);
         args.xslot = exchange->xslot;
@@ -391,9 +392,14 @@ pd_status pd::encode_prefix_maps(const pd_plan &plan, const void *k, const void 
 
 pd_status pd::create_suffix_plan(const pd_layout *layout, const int32_t *table, int64_t table_width,
                                  const int32_t *lengths, const int32_t *max_lengths, const int32_t *first_pages,
-                                 pd_dtype dtype, int32_t device, pd_plan **out_plan) {
-    return create_impl(layout, table, table_width, lengths, max_lengths, 256, 0, dtype, device, 0, out_plan,
+                                 pd_dtype dtype, int32_t device, int32_t num_ctas, pd_plan **out_plan) {
+    return create_impl(layout, table, table_width, lengths, max_lengths, 256, 0, dtype, device, num_ctas, out_plan,
                        first_pages);
+}
+
+pd_status pd::decode_suffix(pd_plan *plan, const void *q, const void *k, const void *v, const int32_t *table,
+                            const int32_t *lengths, float *out, float *stats, bool beside, void *stream) {
+    return decode_impl(plan, q, k, v, plan->dtype, out, stats, stream, table, lengths, nullptr, beside);
 }
 
 PD_API pd_status pd_plan_create(const pd_layout *layout, const int32_t *table, int64_t table_width,

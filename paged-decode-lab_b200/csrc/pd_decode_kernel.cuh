@@ -64,6 +64,10 @@ struct DecodeArgs {
     int32_t num_merge_rows;
     int32_t fused_merge;         // 1: the CTAs merge the partials after a grid barrier
     int32_t pair;                // 1: clusters of two CTAs split each group and merge it themselves
+    // 1: runs beside the kernel before it in the stream, which let this one start once its own
+    // predecessors had finished: q, the caches and the metadata are complete at the start, and the
+    // grid ends no earlier than that kernel (its dependents wait for both)
+    int32_t beside;
     // Dynamic plans: groups cover each sequence up to its capacity (group word
     // 4); the live length of sequence b is min(lengths[b], capacity), pages at
     // or past it are skipped, and page ids always come from `table`.
@@ -1071,7 +1075,8 @@ __global__ void __launch_bounds__((HG * (GT / 8) * NSUB + 1) * 32, 1)
     // Launched programmatically dependent on the previous kernel in the
     // stream: everything above (plan metadata, shared-memory set-up) may
     // overlap its tail; q, the caches and every output wait for it to finish.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.beside) __threadfence();
+    else asm volatile("griddepcontrol.wait;" ::: "memory");
     if (MODE == kModeDecode && a.fused_merge && threadIdx.x == 0) atomicAdd(a.gb.started, 1ull);
     // Exchange mode: this launch's number (1, 2, ...) and the buffer parity it writes.
     const uint32_t xe = a.xworld
@@ -1081,6 +1086,7 @@ __global__ void __launch_bounds__((HG * (GT / 8) * NSUB + 1) * 32, 1)
     if (warp == NC) {
         stream_page_tiles<T, S::TILE_BYTES, S::HALF_BYTES, SLOTS>(&tm_k, &tm_v, a, ring, full_bar, empty_bar,
                                                                 slot_valid, flags, hv, seg_begin, seg_end, lane);
+        if (a.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 

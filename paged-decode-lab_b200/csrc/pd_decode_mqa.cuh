@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(MqaShape<D, T>::THREADS, 1)
     const uint32_t prank = a.pair ? cluster_ctarank() : 0u;
     if (a.pair) cluster_sync_all();
 
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.beside) __threadfence();
+    else asm volatile("griddepcontrol.wait;" ::: "memory");
     if (a.fused_merge && threadIdx.x == 0) atomicAdd(a.gb.started, 1ull);
     const uint32_t xe = a.xworld
         ? __ldcv(reinterpret_cast<const unsigned int *>(a.xpeer[a.xrank] + kXEpochs) + blockIdx.x) + 1u : 0u;
@@ -345,6 +346,7 @@ __global__ void __launch_bounds__(MqaShape<D, T>::THREADS, 1)
             &tm_k, &tm_v, a, kring, vring, kfull, kempty, vfull, vempty, kvalid, vvalid, flags, seg_begin, seg_end,
             lane);
         if (a.pair) cluster_sync_all();   // the partner's merge waits for every thread of both CTAs
+        if (a.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 

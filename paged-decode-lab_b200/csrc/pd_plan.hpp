@@ -92,10 +92,14 @@ pd_status build_plan(const pd_layout *layout, const int32_t *table, int64_t widt
                      int32_t merge_mode, pd_dtype dtype, int32_t num_ctas, int32_t sm_count,
                      pd_plan &plan, bool allow_pair = true, const int32_t *first_pages = nullptr);
 
-// A decode plan of the sequences' pages from first_pages[b] on.
+// A decode plan of the sequences' pages from first_pages[b] on; num_ctas as in pd_plan_create.
 pd_status create_suffix_plan(const pd_layout *layout, const int32_t *table, int64_t width, const int32_t *lengths,
                              const int32_t *max_lengths, const int32_t *first_pages, pd_dtype dtype, int32_t device,
-                             pd_plan **out_plan);
+                             int32_t num_ctas, pd_plan **out_plan);
+
+// Decode such a plan (table and lengths live, or NULL); `beside`: see DecodeArgs.
+pd_status decode_suffix(pd_plan *plan, const void *q, const void *k, const void *v, const int32_t *table,
+                        const int32_t *lengths, float *out, float *stats, bool beside, void *stream);
 
 // One-head page views of the caches as the tcgen05 kernels read them: K in
 // 8-token groups, V token by token.

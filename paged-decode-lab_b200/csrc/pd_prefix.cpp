@@ -128,72 +128,92 @@ struct SimtPlan {
 // streams (see pd_prefix_mma.cuh).
 struct MmaShape {
     static constexpr int64_t rows = 128, step_tokens = 64;
-    // In steps (0.9 us): start and end of a CTA (launch, first loads, rows out); the merge kernel; and
-    // the partials' way through memory, FP32 values a step.
-    static constexpr int64_t overhead_steps = 7, merge_steps = 3, values_per_step = 20 * 128 * 128;
 };
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace
 
-pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count) {
+void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
     const pd_layout &L = p.layout;
-    const int D = L.head_dim;
     const bool mma = p.dtype == PD_FLOAT16;
     p.group = L.query_heads / L.kv_heads;
     int64_t most_rows = 0;
     for (const PrefixGroup &g : p.groups) most_rows = std::max(most_rows, int64_t(g.members.size()) * p.group);
     p.tile_rows = int32_t(mma ? MmaShape::rows : most_rows > 16 ? 64 : 16);
-    const int64_t simt_ctas_per_sm = p.tile_rows == 16 ? 4 : 2;
     p.item_words = mma ? 16 : 8;
+    p.item_steps = 1;
+    p.suffix_ctas = 0;
+    p.shared_us = p.apart_us = 0;
+    if (p.groups.empty()) return;
     const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size;
-    const auto tiles_of = [&](const PrefixGroup &g) {
-        return (int64_t(g.members.size()) * p.group + p.tile_rows - 1) / p.tile_rows;
-    };
-    const auto steps_of = [&](const PrefixGroup &g) { return (g.pages + step_pages - 1) / step_pages; };
-    // FP16: what finishes first when the CTAs run in waves of one per SM and each
-    // costs its steps and the fixed overhead: a CTA per pair of row tiles or per tile
-    // that sees the whole prefix and writes the output (direct), or any number of
-    // pieces that leave partials for the merge kernel.
-    int64_t item_steps = 1;
-    bool pair_tiles = true;
-    p.direct = false;
-    if (mma) {
-        int64_t most = 1, pairs = 0, tiles = 0, best = INT64_MAX;
-        for (const PrefixGroup &g : p.groups) {
-            most = std::max<int64_t>(most, steps_of(g));
-            pairs += L.kv_heads * ((tiles_of(g) + 1) / 2);
-            tiles += L.kv_heads * tiles_of(g);
-        }
-        int64_t values = 0;     // of the partials
-        const auto items = [&](int64_t steps) {     // CTAs of so many steps
-            int64_t n = 0;
-            values = 0;
-            for (const PrefixGroup &g : p.groups) {
-                const int64_t t = tiles_of(g), s = steps_of(g), pieces = (s + steps - 1) / steps;
-                n += L.kv_heads * (t / 2 * pieces + t % 2 * ((pieces + 1) / 2));
-                values += L.query_heads * int64_t(g.members.size()) * D * pieces;
-            }
-            return n;
-        };
-        const auto waves = [&](int64_t ctas) { return (ctas + sm_count - 1) / sm_count; };
-        for (int64_t steps = 1; steps <= most; ++steps) {
-            const int64_t n = items(steps);
-            const int64_t cost = waves(n) * (MmaShape::overhead_steps + steps) + MmaShape::merge_steps +
-                                 values / MmaShape::values_per_step;
-            if (cost < best) best = cost, item_steps = steps;
-        }
-        const int64_t by_pair = waves(pairs) * (MmaShape::overhead_steps + most);
-        const int64_t by_tile = waves(tiles) * (MmaShape::overhead_steps + (most + 1) / 2);
-        if (by_pair <= best || by_tile <= best) {
-            p.direct = !p.groups.empty();
-            pair_tiles = by_pair <= by_tile;
-            item_steps = most;
-        }
-    } else {
+    const auto tiles_of = [&](const PrefixGroup &g) { return ceil_div(int64_t(g.members.size()) * p.group, p.tile_rows); };
+    const auto steps_of = [&](const PrefixGroup &g) { return ceil_div(g.pages, step_pages); };
+    // What the decode kernel alone would take (us, measured on a B200): 12 and its bytes, the copies of
+    // shared pages from L2.
+    const double page_bytes = (mma ? 4.0 : 8.0) * L.page_size * L.kv_heads * L.head_dim;
+    int64_t copies = 0, shared_pages = 0;
+    double flops = 0;
+    for (const PrefixGroup &g : p.groups) {
+        copies += int64_t(g.members.size()) * g.pages;
+        shared_pages += g.pages;
+        flops += 4.0 * L.kv_heads * double(tiles_of(g) * p.tile_rows) * g.pages * L.page_size * L.head_dim;
+    }
+    p.apart_us = 12 + suffix_pages * page_bytes / 5.5e6 +
+                 copies * page_bytes / (!mma ? 9e6 : p.group > 16 ? 7.5e6 : 14e6);
+    if (!mma) {
         int64_t work = 0;
         for (const PrefixGroup &g : p.groups) work += L.kv_heads * tiles_of(g) * steps_of(g);
-        item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, simt_ctas_per_sm * sm_count));
+        p.item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, (p.tile_rows == 16 ? 4 : 2) * sm_count));
+        p.shared_us = 22 + suffix_pages * page_bytes / 5.5e6 +
+                      std::max(shared_pages * page_bytes / 5e6, flops / (p.tile_rows == 16 ? 15e6 : 23e6));
+        return;
     }
+    // Times in us (measured on a B200).  A CTA of the prefix kernel takes 7 for its start and end and
+    // 0.94 a step; the prefix's bytes come at 6.2e6 B/us at best.  The decode kernel takes 9 and its
+    // bytes at 5.5e6 B/us, or 48e3 per SM, and 3 for each sequence on an SM.  The merge takes 3 and 350e3 FP32 values of partials a
+    // us.  The two kernels run beside each other where both fit and that is sooner done.  (256
+    // sequences of 64:8 heads, 4096 shared and 512 own tokens each: 64 CTAs beside 84 136 us, 128 and then
+    // 148 174, 128 beside 20 364.)
+    int64_t most = 1;
+    for (const PrefixGroup &g : p.groups) most = std::max(most, steps_of(g));
+    const double segments = double(L.batch) * ceil_div(L.kv_heads, 8) * ceil_div(p.group, 32);
+    const auto suffix_us = [&](int64_t sms) {
+        return suffix_pages == 0
+                   ? 0.0
+                   : 9 + suffix_pages * page_bytes / std::min(5.5e6, 48e3 * double(sms)) + 3 * segments / double(sms);
+    };
+    double best = 1e300;
+    for (int64_t steps = 1; steps <= most; ++steps) {
+        int64_t ctas = 0, values = 0;
+        for (const PrefixGroup &g : p.groups) {
+            const int64_t tiles = tiles_of(g), pieces = ceil_div(steps_of(g), steps);
+            ctas += L.kv_heads * (tiles / 2 * pieces + tiles % 2 * ceil_div(pieces, 2));
+            values += L.query_heads * int64_t(g.members.size()) * L.head_dim * pieces;
+        }
+        const double prefix = std::max(0.94 * double(ceil_div(ctas, sm_count) * (7 + steps)),
+                                       7 + shared_pages * page_bytes / 6.2e6);
+        const double behind = prefix + suffix_us(sm_count);
+        const double beside =
+            suffix_pages > 0 && ctas < sm_count ? std::max(prefix, suffix_us(sm_count - ctas)) : behind;
+        const double us = std::min(beside, behind) + 3 + double(values) / 350e3;
+        if (us < best) {
+            best = us;
+            p.shared_us = us + 4;
+            p.item_steps = steps;
+            p.suffix_ctas = beside < behind ? int32_t(sm_count - ctas) : 0;
+        }
+    }
+}
+
+pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count) {
+    const pd_layout &L = p.layout;
+    const int D = L.head_dim;
+    const bool mma = p.dtype == PD_FLOAT16;
+    const int64_t item_steps = p.item_steps;
+    const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size;
+    const auto tiles_of = [&](const PrefixGroup &g) { return ceil_div(int64_t(g.members.size()) * p.group, p.tile_rows); };
+    const auto steps_of = [&](const PrefixGroup &g) { return ceil_div(g.pages, step_pages); };
     p.seqs.assign(size_t(L.batch) * 8, 0);
     for (int b = 0; b < L.batch; ++b) p.seqs[size_t(b) * 8] = -1;
     p.items.clear();
@@ -219,11 +239,10 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
         };
         for (int h = 0; h < L.kv_heads; ++h) {
             for (int64_t t = 0; t < ntiles; ++t) {
-                const bool paired = mma && pair_tiles && (t ^ 1) < ntiles;
+                const bool paired = mma && (t ^ 1) < ntiles;
                 const bool split = mma && !paired && steps > 1;
-                int64_t pieces = (steps + item_steps - 1) / item_steps;
-                if (split) pieces = (steps + 2 * item_steps - 1) / (2 * item_steps) * 2;
-                pieces = std::min(pieces, steps);
+                int64_t pieces = ceil_div(steps, item_steps);
+                if (split) pieces = std::min(steps, ceil_div(pieces, 2) * 2);
                 p.tiles.insert(p.tiles.end(), {int32_t(slots), int32_t(pieces)});
                 const int32_t slot = int32_t(slots), tile = int32_t(t);
                 slots += pieces;
@@ -244,14 +263,14 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
                                 std::swap(sx, sy);
                             }
                         }
-                        p.items.insert(p.items.end(), {m0, n, h, 0, pg, g.pages, 0, 0, tile, x[0], x[1], sx, tile, x[2],
+                        p.items.insert(p.items.end(), {m0, n, h, 0, pg, 0, 0, 0, tile, x[0], x[1], sx, tile, x[2],
                                                        x[3], sy});
                     }
                 } else if (t % 2) {
                     // both tiles of a pair have the same pieces; this one's slots follow the other's
                     for (int64_t c = 0; c < pieces; ++c)
                         p.items.insert(p.items.end(),
-                                       {m0, n, h, 1, pg, g.pages, 0, 0, tile - 1, bound(c, pieces), bound(c + 1, pieces),
+                                       {m0, n, h, 1, pg, 0, 0, 0, tile - 1, bound(c, pieces), bound(c + 1, pieces),
                                         int32_t(slot - pieces + c), tile, bound(c, pieces), bound(c + 1, pieces),
                                         int32_t(slot + c)});
                 }
@@ -260,17 +279,6 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
         members.insert(members.end(), g.members.begin(), g.members.end());
         const int32_t *row = table + int64_t(g.members[0]) * p.width;
         pages.insert(pages.end(), row, row + g.pages);
-    }
-    if (p.direct) {
-        // every row is written by the prefix kernel: sequences of no group, four to a CTA
-        slots = 0;
-        const size_t first = members.size();
-        for (int b = 0; b < L.batch; ++b)
-            if (p.seqs[size_t(b) * 8] < 0) members.push_back(b);
-        for (size_t at = first; at < members.size(); at += 4) {
-            p.items.insert(p.items.end(), {int32_t(at), int32_t(std::min<size_t>(4, members.size() - at)), 0, 2});
-            p.items.insert(p.items.end(), 12, 0);
-        }
     }
     p.slots = int32_t(slots);
     // Merge: at most four pieces (one batch of loads) per thread set, while the

@@ -53,9 +53,7 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
     using S = SimtShape<R, D>;
     constexpr int N = kSimtTokens, TR = R / 16, OR = R / 8, OD = D / 16;   // rows and dims of a thread's blocks
     extern __shared__ __align__(16) float sm[];
-    // With a suffix decode in front, q, the caches and the lengths are complete (it waited for
-    // their writers before any of this grid's CTAs could start) and only its rows are not.
-    if (!a.rows) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 i0 = a.items[2 * blockIdx.x], i1 = a.items[2 * blockIdx.x + 1];
     const int T = a.page_size, tid = threadIdx.x, end = i1.z * T;
     const uint32_t base = smem_u32(sm);
@@ -189,8 +187,6 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
                 make_ulonglong2(o[i][2 * k], o[i][2 * k + 1]);
         }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // the suffix decode's rows are complete when this grid is
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Each output row from the suffix's normalised row and the prefix pieces: D / 8
@@ -328,17 +324,17 @@ cudaError_t allow_smem(const pd_prefix_plan &p) {
 template <int D>
 cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CUtensorMap &map_k,
                           const CUtensorMap &map_v, cudaStream_t stream) {
-    cudaError_t err = cudaSuccess;
     const int64_t items = int64_t(p.items.size()) / p.item_words;
-    if (items && p.dtype == PD_FLOAT16) {
+    if (p.dtype == PD_FLOAT16) {
         const MmaEntry e = mma_entry_for(p.layout);
-        err = launch_dependent(e.kernel, items, e.threads, e.smem, stream, map_k, map_v, a);
-        if (p.direct) return err;
-    } else if (items) {
-        const SimtEntry e = simt_entry<D>(p.tile_rows);
-        err = launch_dependent(e.kernel, items, kSimtThreads, e.smem, stream, a);
+        return launch_dependent(e.kernel, items, e.threads, e.smem, stream, map_k, map_v, a);
     }
-    if (err != cudaSuccess) return err;
+    const SimtEntry e = simt_entry<D>(p.tile_rows);
+    return launch_dependent(e.kernel, items, kSimtThreads, e.smem, stream, a);
+}
+
+template <int D>
+cudaError_t launch_merge(const pd_prefix_plan &p, const PrefixArgs &a, cudaStream_t stream) {
     const int64_t rows = int64_t(a.B) * a.Hq, per_cta = kMergeThreads / (D / 8) / p.merge_ways;
     const int64_t grid = (rows + per_cta - 1) / per_cta;
     return p.dtype == PD_FLOAT16
@@ -381,49 +377,43 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.group = p->group;
     a.page_size = p->layout.page_size;
     a.tile_rows = p->tile_rows;
-    a.direct = p->direct ? 1 : 0;
     a.P = p->layout.physical_pages;
     a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(p->layout.head_dim)));
+    // The prefix kernel goes first: it lets the suffix's decode start beside it as soon as its own
+    // CTAs have (FP16, on the SMs it leaves), and the merge waits for both.
     pd_status s = PD_OK;
-    if (p->items.empty() && dtype == PD_FLOAT32) {      // nothing shared, nothing to convert
-        s = table ? pd_decode_dynamic(p->suffix, q, k, v, dtype, table, lengths, static_cast<float *>(out), nullptr, stream)
-                  : pd_decode(p->suffix, q, k, v, dtype, static_cast<float *>(out), stream);
-        if (prev >= 0 && prev != p->device) cudaSetDevice(prev);
-        return s;
+    const auto st = static_cast<cudaStream_t>(stream);
+    const bool wide = p->layout.head_dim == 128;
+    if (!p->items.empty()) {
+        alignas(64) CUtensorMap map_k, map_v;
+        if (dtype == PD_FLOAT16) s = encode_prefix_maps(*p->suffix, k, v, &map_k, &map_v);
+        if (s == PD_OK) {
+            err = wide ? launch_prefix<128>(*p, a, map_k, map_v, st) : launch_prefix<64>(*p, a, map_k, map_v, st);
+            if (err != cudaSuccess) s = fail(PD_ERR_CUDA, std::string("prefix launch: ") + cudaGetErrorString(err));
+        }
     }
-    alignas(64) CUtensorMap map_k, map_v;
-    if (dtype == PD_FLOAT16 && !p->items.empty()) s = encode_prefix_maps(*p->suffix, k, v, &map_k, &map_v);
-    if (s == PD_OK && !p->suffix_empty) {
-        float *rows = reinterpret_cast<float *>(p->dev + im.off_rows);
+    const bool merges = !p->items.empty() || dtype == PD_FLOAT16;     // (else: nothing shared, nothing to convert)
+    if (s == PD_OK && (!p->suffix_empty || !merges)) {
+        float *rows = merges ? reinterpret_cast<float *>(p->dev + im.off_rows) : static_cast<float *>(out);
         float *stats = reinterpret_cast<float *>(p->dev + im.off_stats);
-        s = table ? pd_decode_dynamic(p->suffix, q, k, v, dtype, table, lengths, rows, stats, stream)
-                  : pd_decode_with_stats(p->suffix, q, k, v, dtype, rows, stats, stream);
+        s = decode_suffix(p->suffix, q, k, v, table, lengths, rows, stats, !p->items.empty() && p->suffix_ctas > 0, stream);
         a.rows = rows;
         a.stats = stats;
     }
-    if (s == PD_OK) {
-        const auto st = static_cast<cudaStream_t>(stream);
-        err = p->layout.head_dim == 64 ? launch_prefix<64>(*p, a, map_k, map_v, st)
-                                       : launch_prefix<128>(*p, a, map_k, map_v, st);
-        if (err != cudaSuccess) s = fail(PD_ERR_CUDA, std::string("prefix launch: ") + cudaGetErrorString(err));
+    if (s == PD_OK && merges) {
+        err = wide ? launch_merge<128>(*p, a, st) : launch_merge<64>(*p, a, st);
+        if (err != cudaSuccess) s = fail(PD_ERR_CUDA, std::string("merge launch: ") + cudaGetErrorString(err));
     }
     if (prev >= 0 && prev != p->device) cudaSetDevice(prev);
     return s;
 }
-
-// Found groups are used where they save reading this much again.  The decode
-// kernel reads a shared page's copies from L2 at about 13 TB/s, and the prefix and merge
-// kernels cost about 20 us.  Measured, us shared / not: 32 sequences of 32:8 FP16 heads behind 1024,
-// 2048 and 4096 tokens (130, 260 and 520 MB) 30 / 24, 32 / 34, 36 / 53; 64 of 32:1 behind 2048
-// and 8192 (66, 264 MB) 32 / 19, 44 / 46; 16 of 32:8 FP32 behind 2048 and 4096 (252, 503 MB) 51 / 49, 71 / 85.
-constexpr int64_t kWorthBytes = int64_t(256) << 20;
 
 pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t width, const int32_t *lengths,
                       const int32_t *max_lengths, int32_t group_count, const int32_t *indptr, const int32_t *members,
                       const int32_t *pages, pd_dtype dtype, int32_t device, pd_prefix_plan &p) {
     // the decode plan's own checks of layout, table and lengths, before the groups look at them
     pd_plan *whole = nullptr;
-    pd_status s = create_suffix_plan(layout, table, width, lengths, max_lengths, nullptr, dtype, -1, &whole);
+    pd_status s = create_suffix_plan(layout, table, width, lengths, max_lengths, nullptr, dtype, -1, 0, &whole);
     if (s != PD_OK) return s;
     pd_plan_destroy(whole);
     p.layout = *layout;
@@ -433,11 +423,6 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t wid
     p.dynamic = max_lengths != nullptr;
     if (group_count < 0) {
         find_prefix_groups(p.layout, table, width, lengths, p.groups);
-        int64_t saved = 0;
-        for (const PrefixGroup &g : p.groups) saved += int64_t(g.members.size() - 1) * g.pages;
-        const int64_t page_bytes = 2 * int64_t(layout->page_size) * layout->kv_heads * layout->head_dim *
-                                   (dtype == PD_FLOAT16 ? 2 : 4);
-        if (group_count == -1 && saved * page_bytes < kWorthBytes) p.groups.clear();
     } else {
         if (group_count > 0 && (!indptr || !members || !pages))
             return fail(PD_ERR_VALUE, "group arrays must not be NULL");
@@ -451,13 +436,32 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t wid
         }
         if ((s = check_prefix_groups(p.layout, table, width, lengths, p.groups)) != PD_OK) return s;
     }
+    int sm_count = 148;
+    if (device >= 0) {
+        const cudaError_t err = cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device);
+        if (err != cudaSuccess) return fail(PD_ERR_CUDA, std::string("device query: ") + cudaGetErrorString(err));
+    }
     std::vector<int32_t> first(layout->batch, 0);
-    for (const PrefixGroup &g : p.groups)
-        for (const int32_t b : g.members) first[b] = g.pages;
-    s = create_suffix_plan(layout, table, width, lengths, max_lengths, first.data(), dtype, device, &p.suffix);
+    const auto choose = [&]() {
+        std::fill(first.begin(), first.end(), 0);
+        for (const PrefixGroup &g : p.groups)
+            for (const int32_t b : g.members) first[b] = g.pages;
+        const int32_t *span = max_lengths ? max_lengths : lengths;
+        int64_t suffix_pages = 0;
+        for (int b = 0; b < layout->batch; ++b)
+            suffix_pages += std::max<int64_t>(0, (int64_t(span[b]) + layout->page_size - 1) / layout->page_size - first[b]);
+        p.suffix_empty = suffix_pages == 0;
+        choose_pieces(p, suffix_pages, sm_count);
+    };
+    choose();
+    if (group_count == -1 && p.shared_us >= p.apart_us) {   // sharing would not pay
+        p.groups.clear();
+        choose();
+    }
+    s = create_suffix_plan(layout, table, width, lengths, max_lengths, first.data(), dtype, device, p.suffix_ctas,
+                           &p.suffix);
     if (s != PD_OK) return s;
-    p.suffix_empty = p.suffix->total_pages == 0;
-    return build_prefix_plan(p, table, lengths, p.suffix->sm_count);
+    return build_prefix_plan(p, table, lengths, sm_count);
 }
 
 }  // namespace
@@ -501,7 +505,7 @@ PD_API pd_status pd_prefix_plan_get_info(const pd_prefix_plan *p, pd_prefix_info
     info->tile_rows = p->tile_rows;
     info->items = int32_t(p->items.size() / p->item_words);
     info->item_words = p->item_words;
-    info->direct = p->direct ? 1 : 0;
+    info->suffix_ctas = p->suffix_ctas;
     info->suffix_launch = p->suffix_empty ? 0 : 1;
     info->dynamic = p->dynamic ? 1 : 0;
     info->device_bytes = int64_t(p->image.bytes);

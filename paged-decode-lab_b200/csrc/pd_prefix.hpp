@@ -34,7 +34,9 @@ struct pd_prefix_plan {
     int32_t group = 0;              // G = Hq / Hkv
     int32_t tile_rows = 0;          // query rows of one prefix tile
     int32_t slots = 0;              // partial slots (tile pieces)
-    bool direct = false;            // FP16: the prefix kernel writes the output, no partials or merge kernel
+    double shared_us = 0, apart_us = 0;   // estimates: with these groups, without any
+    int64_t item_steps = 1;         // steps of the longest work item (choose_pieces)
+    int32_t suffix_ctas = 0;        // SMs left to the suffix's decode beside the prefix kernel, 0: it runs behind it
     int32_t merge_ways = 1;         // thread sets that share a row's pieces in the merge
     bool dynamic = false;
     bool suffix_empty = false;      // no sequence has pages past its prefix: nothing for the decode kernel
@@ -63,8 +65,11 @@ void find_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t w
 pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,
                               const std::vector<PrefixGroup> &groups);
 
-// Lay the groups' work out over the device and build the device image; the
-// suffix plan is set.
+// How the groups' work is cut (item_steps) and which SMs the suffix gets
+// (suffix_ctas), from the groups and the suffix's pages.
+void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count);
+
+// Lay the groups' work out and build the device image; the suffix plan is set.
 pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count);
 
 }  // namespace pd

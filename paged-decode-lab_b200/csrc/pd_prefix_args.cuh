@@ -6,17 +6,16 @@
 
 namespace pd {
 
-// FP16 work items: two streams over their own pages, two over the same pages, or
-// sequences of no group (`members` of them) whose rows only change type.
-enum : int { kItemSplit = 0, kItemPaired = 1, kItemCopy = 2 };
+// FP16 work items: two streams over their own pages of one row tile, or two row tiles over the same pages.
+enum : int { kItemSplit = 0, kItemPaired = 1 };
 
 struct PrefixArgs {
     const void *q;              // [B, Hq, D]
     const void *k, *v;          // [P, T, Hkv, D]
     // Work items.  FP32: 2 words of 4: {first member, members, KV head, row tile}, {first of the
     // group's pages in `pages`, first and end page of the piece, partial slot}.  FP16: 4 of them:
-    // {first member, members, KV head, kind}, {first of the group's pages in `pages`, shared pages,
-    // 0, 0}, and per stream {row tile, first page, end page, slot}; kind kItem*.
+    // {first member, members, KV head, kind}, {first of the group's pages in `pages`, 0, 0, 0},
+    // and per stream {row tile, first page, end page, slot}; kind kItem*.
     const int4 *items;
     // Per sequence: {member index in its group or -1, first row tile of KV head 0, row tiles per KV
     // head, first of the group's pages in `pages`}, {shared pages, 0, 0, 0}.
@@ -32,7 +31,6 @@ struct PrefixArgs {
     void *out;                  // [B, Hq, D]
     uint32_t *error;
     int32_t B, Hq, Hkv, group, page_size, tile_rows;
-    int32_t direct;             // FP16: the prefix kernel writes the output (0: partials)
     int64_t P;
     float scale_log2;           // log2(e) / sqrt(D)
 };

@@ -30,13 +30,9 @@
 // are dropped (a live length inside the prefix: the merge kernel's slow path),
 // so no scores need masks; a last step of fewer pages takes fewer columns.
 //
-// The end of an item.  In a direct plan (enough row tiles to fill the device) the
-// CTA has seen the whole prefix of its rows, merges them with the suffix and writes
-// the output: paired streams each their own rows, split streams (the two halves
-// of one tile's prefix, both outputs in the same tensor-memory lanes) half of the head
-// dims each.  Otherwise each stream leaves its rows' (m, l, o) as a partial for the
-// merge kernel.  (Merging the pieces of a tile inside a cluster measured slower than
-// that kernel: 64 KB a stream through distributed shared memory or L2 took 3-6 us.)
+// Each stream leaves its rows' (m, l, o) as a partial for the merge kernel.  The
+// grid is kept smaller than the device: once its CTAs have started, the suffix's decode
+// kernel runs beside it on the other SMs.
 //
 // Every wait is bounded; on a timeout the CTA records PD_DEVERR_TIMEOUT,
 // unwinds, waits for its own MMAs and copies and frees its tensor memory.
@@ -45,7 +41,6 @@
 #include "paged_decode.h"
 #include "pd_device.cuh"
 #include "pd_prefix_args.cuh"
-#include "pd_prefix_merge.cuh"
 #include "pd_tcgen05.cuh"
 
 namespace pd {
@@ -66,8 +61,8 @@ struct PrefixShape {
     // tensor memory: score blocks (weights in their first half) [stream][2], outputs [stream]
     static constexpr int S_COL = 0, O_COL = 4 * NS;
     static constexpr int TMEM_COLS = 512;
-    static constexpr int NBARS = 2 * SLOTS + 2 + 4 + 4 + 2 + 2 + 1;   // + 16 bytes of flags
-    static constexpr size_t SMEM = 1024 + 2 * size_t(Q_BYTES) + size_t(SLOTS) * STEP_BYTES + NBARS * 8 + 16 + 2 * M * 4;
+    static constexpr int NBARS = 2 * SLOTS + 2 + 4 + 4 + 2 + 2 + 1;
+    static constexpr size_t SMEM = 1024 + 2 * size_t(Q_BYTES) + size_t(SLOTS) * STEP_BYTES + NBARS * 8 + 16;
     static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory budget");
     static_assert(SMEM <= 232448 && SMEM > 116 * 1024, "one CTA per SM: tensor memory is never contended");
 };
@@ -84,13 +79,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// 32 bytes past L1: a whole sector by one thread.
-__device__ __forceinline__ void load_sector(uint32_t *r, const void *p) {
-    asm volatile("ld.global.cg.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "l"(p)
-                 : "memory");
-}
+// 32 bytes: a whole sector by one thread.
 __device__ __forceinline__ void store_sector(void *p, const uint32_t *r) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -105,7 +94,7 @@ struct PrefixStream {
 
 struct PrefixItem {
     int member0, members, head, kind;
-    int page0, pages;
+    int page0;
     PrefixStream s0, s1;            // an absent stream has end == first
     __device__ __forceinline__ PrefixStream s(int t) const {
         return PrefixStream{t ? s1.tile : s0.tile, t ? s1.first : s0.first, t ? s1.end : s0.end, t ? s1.slot : s0.slot};
@@ -117,7 +106,7 @@ __device__ __forceinline__ PrefixItem prefix_item(const PrefixArgs &a, int i) {
     const int4 z = __ldg(a.items + 4 * i + 2), w = __ldg(a.items + 4 * i + 3);
     PrefixItem it;
     it.member0 = x.x, it.members = x.y, it.head = x.z, it.kind = x.w;
-    it.page0 = y.x, it.pages = y.y;
+    it.page0 = y.x;
     it.s0 = PrefixStream{z.x, z.y, z.z, z.w};
     it.s1 = PrefixStream{w.x, w.y, w.z, w.w};
     return it;
@@ -167,8 +156,6 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     uint64_t *mma_done = o_last + 2;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(mma_done + 1);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1) + 1;
-    int32_t *out_rows = reinterpret_cast<int32_t *>(mma_done + 3);     // [2][128] output rows, see below
-    float2 *row_ml = reinterpret_cast<float2 *>(qbuf + S::Q_BYTES);    // [2][128] (m, l) of split streams (one query tile)
 
     const int warp = int(__reduce_max_sync(kFullMask, threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const PrefixItem it = prefix_item(a, blockIdx.x);
@@ -177,20 +164,6 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     // Warps 8 to 11 stay converged, and what they hand to the hardware is the same in all lanes
     // (reductions over the warp give the compiler the proof): operands then live in uniform registers.
     const auto uniform = [](int x) { return __reduce_max_sync(kFullMask, x); };
-    if (it.kind == kItemCopy) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int lanes = a.Hq * (D / 8);
-        for (int e = threadIdx.x; e < it.members * lanes; e += S::THREADS) {
-            const int64_t row = int64_t(__ldg(a.members + it.member0 + e / lanes)) * a.Hq + e % lanes / (D / 8);
-            RowSum sum(0.f);
-            if (a.rows) {
-                const float4 *x = reinterpret_cast<const float4 *>(a.rows + row * D + e % (D / 8) * 8);
-                sum.add(make_float2(0.f, 1.f), __ldcg(x), __ldcg(x + 1));
-            }
-            store_row<__half, D>(sum, a, row, e % (D / 8));
-        }
-        return;
-    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < SLOTS; ++s) {
             mbar_init(smem_u32(full + s), 1);
@@ -217,9 +190,8 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    // With a suffix decode in front, q, the caches and the lengths are complete (it waited for
-    // their writers before any CTA of this grid could start) and only its rows are not.
-    if (!a.rows) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const auto fail_wait = [&]() {
         if (!*abort_flag) atomicOr(a.error, PD_DEVERR_TIMEOUT);
@@ -377,15 +349,6 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(q_full + t));
         }
-        // where the row goes in a direct plan: -1 nowhere, -2 - row a sequence that ends inside its prefix
-        int row = -1;
-        if (a.direct && (st.tile * S::M + r) / a.group < it.members) {
-            const int gr = st.tile * S::M + r;
-            const int b = __ldg(a.members + it.member0 + gr / a.group);
-            row = b * a.Hq + it.head * a.group + gr % a.group;
-            if (__ldcg(a.lengths + b) < it.pages * a.page_size) row = -2 - row;
-        }
-        out_rows[t * S::M + r] = row;
         const uint32_t lanes = uint32_t(32 * quad) << 16;
         const uint32_t ts = tmem + lanes + S::S_COL + 2 * t * S::NS, to = tmem + lanes + S::O_COL + t * D;
         const auto warp_wait = [&](uint64_t *bar, int parity) {
@@ -479,56 +442,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         tc::fence_after_sync();
         const float2 l = unpack_f32x2(add_f32x2(l2, l3));
         const bool on = n > 0 && ok && (st.tile * S::M + r) / a.group < it.members;
-        if (a.direct) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            // stream u's (m, l) of the row: own, and in a split item the other's as well
-            float2 ml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
-            ml[t] = on ? make_float2(m, l.x + l.y) : ml[t];
-            if (!paired) {
-                row_ml[t * S::M + r] = ml[t];
-                tc::fence_before_sync();
-                named_barrier_sync(1, 2 * S::M);
-                tc::fence_after_sync();
-                ml[0] = row_ml[r], ml[1] = row_ml[S::M + r];
-            }
-            const bool live = row >= 0;
-            const float2 suffix = live ? suffix_stats(a, row) : make_float2(-INFINITY, 0.f);
-            const float top = fmaxf(fmaxf(top_of(ml[0]), top_of(ml[1])), top_of(suffix));
-            const auto weight = [&](float2 x) { return x.y != 0.f ? exp2f(x.x - top) : 0.f; };
-            const float w0 = weight(ml[0]), w1 = weight(ml[1]), ws = weight(suffix) * suffix.y;
-            const float den = fmaf(w0, ml[0].y, fmaf(w1, ml[1].y, ws));
-            const float inv = den != 0.f ? 1.f / den : 0.f;
-            const float f0 = w0 * inv, f1 = w1 * inv, fs = ws * inv;
-            const int dims = paired ? D : D / 2, d0 = paired ? 0 : t * dims;
-            const uint32_t o0 = tmem + lanes + S::O_COL + (paired ? t * D : 0) + d0, o1 = o0 + (paired ? 0 : D);
-            const float g0 = paired ? (t ? f1 : f0) : f0, g1 = paired ? 0.f : f1;
-#pragma unroll 1
-            for (int c = 0; c < dims; c += 16) {
-                uint32_t x[16], y[16], z[16];
-                tc::ld_32x32b_x16(o0 + c, x);
-                if (!paired) tc::ld_32x32b_x16(o1 + c, y);
-                if (fs != 0.f) {
-                    load_sector(z, a.rows + int64_t(row) * D + d0 + c);
-                    load_sector(z + 8, a.rows + int64_t(row) * D + d0 + c + 8);
-                }
-                tc::wait_ld();
-                uint32_t packed[8];
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    float v[2];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        // (a part that was never computed holds anything: no factor, no term)
-                        float sum = g0 != 0.f ? __uint_as_float(x[e + k]) * g0 : 0.f;
-                        if (g1 != 0.f) sum = fmaf(__uint_as_float(y[e + k]), g1, sum);
-                        if (fs != 0.f) sum = fmaf(__uint_as_float(z[e + k]), fs, sum);
-                        v[k] = sum;
-                    }
-                    packed[e / 2] = pack_half2(v[0], v[1]);
-                }
-                if (live) store_sector(static_cast<__half *>(a.out) + int64_t(row) * D + d0 + c, packed);
-            }
-        } else if (n > 0) {
+        if (n > 0) {
             // partials lie [D / 8][rows][8]: a row's reads take whole sectors, as do a thread's stores
             float *dst = a.part_o + (int64_t(st.slot) * D * S::M + r * 8);
 #pragma unroll 1
@@ -545,21 +459,9 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         }
         tc::fence_before_sync();
     }
-    if (a.direct) {
-        // rows of sequences that end inside their prefix: D / 8 threads each
-        __syncthreads();
-        for (int x = threadIdx.x / (D / 8); x < (paired ? 2 : 1) * S::M; x += S::THREADS / (D / 8)) {
-            const int own = -2 - out_rows[x];
-            if (own >= 0)
-                row_inside<__half, D>(a, own, it.head, a.pages + it.page0, own / a.Hq, threadIdx.x % (D / 8));
-        }
-    }
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __syncthreads();
     tc::fence_after_sync();
     if (warp == S::W_MMA) tc::dealloc(tmem, S::TMEM_COLS);
-    // the suffix decode's rows are complete when this grid is
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace pd

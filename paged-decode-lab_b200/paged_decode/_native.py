@@ -42,7 +42,7 @@ class PlanInfo(ctypes.Structure):
 
 class PrefixInfo(ctypes.Structure):
     _fields_ = [("groups", ctypes.c_int32), ("members", ctypes.c_int32), ("tile_rows", ctypes.c_int32),
-                ("items", ctypes.c_int32), ("item_words", ctypes.c_int32), ("direct", ctypes.c_int32),
+                ("items", ctypes.c_int32), ("item_words", ctypes.c_int32), ("suffix_ctas", ctypes.c_int32),
                 ("suffix_launch", ctypes.c_int32), ("dynamic", ctypes.c_int32),
                 ("shared_pages", ctypes.c_int64), ("device_bytes", ctypes.c_int64)]
 

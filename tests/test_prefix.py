@@ -200,16 +200,15 @@ def test_dead_rows_of_a_live_length_inside_the_prefix():
     close(out, *exact(q, k, v, table, live))
 
 
-@pytest.mark.parametrize("members,pages,heads,kv,direct", [
-    (400, 32, 64, 8, 1),      # more row tiles than SMs: a CTA per pair of them, and one odd tile
-    (200, 32, 64, 8, 1),      # a CTA per tile
-    (64, 512, 32, 1, 0),      # pairs of tiles in pieces
-    (40, 700, 8, 2, 0)])      # odd tile counts in pieces
-def test_every_way_to_cut_the_work(members, pages, heads, kv, direct):
+@pytest.mark.parametrize("members,pages,heads,kv", [
+    (400, 32, 64, 8),      # more row tiles than SMs, an odd one among them
+    (200, 32, 64, 8),
+    (64, 512, 32, 1),      # pairs of tiles in pieces
+    (40, 700, 8, 2)])      # odd tile counts in pieces
+def test_every_way_to_cut_the_work(members, pages, heads, kv):
     layout, table, lengths, groups, q, k, v = case([(pages, [i % 40 for i in range(members)])], [7, 0], heads, kv, 128,
                                                    16, F16)
     plan = SharedPrefixPlan(layout, table, lengths, prefixes=groups)
-    assert plan.info.direct == direct
     out = plan.run(q, k, v)
     some = np.r_[0:members + 2:9, members, members + 1]
     close(out[some], *exact(q[some], k, v, table[some], lengths[some]))
@@ -219,11 +218,10 @@ def test_every_way_to_cut_the_work(members, pages, heads, kv, direct):
 
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_live_lengths_inside_a_long_prefix(dtype):
-    """As above where the prefix is cut in pieces for the merge kernel."""
+    """As above where the prefix is cut in many pieces."""
     layout, table, lengths, members, q, k, v = case([(600, [4, 0, 9, 20])], [12, 0], 8, 2, 128, 16, dtype)
     k[k.isnan()], v[v.isinf()] = 0.25, 0.5
     plan = SharedPrefixPlan(layout, table, lengths, prefixes=members, dtype=dtype, max_lengths=lengths)
-    assert not plan.info.direct
     live = lengths.copy()
     a, b, c, _ = members[0][0]
     live[a], live[b], live[c] = 0, 1, 9000

@@ -146,7 +146,7 @@ def test_work_items_cover_every_row_and_page_once(dtype, heads, kv, page, counts
     layout, table, lengths, members = shared_batch(counts, others, heads, kv, page)
     info, groups, items = inspect_prefix_plan(layout, table, lengths, prefixes=members, dtype=dtype)
     assert len(items) == info["items"] and info["members"] == sum(n for n, _ in counts)
-    rows_per_tile, seen, copied, slots = info["tile_rows"], {}, 0, []
+    rows_per_tile, seen, slots = info["tile_rows"], {}, []
     first_member, first_page = 0, 0
     starts = {}                                      # the group of a first member
     for g, (n, pages) in enumerate(counts):
@@ -155,16 +155,11 @@ def test_work_items_cover_every_row_and_page_once(dtype, heads, kv, page, counts
     streams = []                                     # (group, head, tile, first, end, slot)
     for it in items:
         it = [int(x) for x in it]
-        if info["item_words"] == 16 and it[3] == 2:
-            assert it[0] >= first_member and 1 <= it[1] <= 4
-            copied += it[1]
-            continue
         g, page0 = starts[it[0]]
         assert it[1] == counts[g][0] and it[4] == page0
         if info["item_words"] == 8:
             streams.append((g, it[2], it[3], it[5], it[6], it[7]))
             continue
-        assert it[5] == counts[g][1]
         a, b = it[8:12], it[12:16]
         if it[3] == 1:                               # two tiles, one run
             assert b[0] == a[0] + 1 and a[1:3] == b[1:3]
@@ -180,10 +175,9 @@ def test_work_items_cover_every_row_and_page_once(dtype, heads, kv, page, counts
         slots.append(slot)
     want = sum(kv * -(-n * (heads // kv) // rows_per_tile) * pages for n, pages in counts)
     assert len(seen) == want
-    if info["direct"]:
-        assert copied == others                      # every row of the batch is written
-    else:
-        assert copied == 0 and sorted(slots) == list(range(len(slots)))
+    assert sorted(slots) == list(range(len(slots)))
+    if info["suffix_ctas"]:                          # the two kernels' CTAs are all resident at once
+        assert info["suffix_launch"] and info["suffix_ctas"] + info["items"] <= 148
 
 
 def test_sharing_is_left_out_where_it_saves_little():
