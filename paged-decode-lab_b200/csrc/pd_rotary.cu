@@ -7,6 +7,12 @@
 // where a pair is (y[i], y[i + r/2]) or, interleaved, (y[2i], y[2i + 1]);
 // y[r:] passes.  Everything in FP32, one rounding at the store.  Appended
 // values are copied bit for bit.
+//
+// Bound by memory: each head row is read and written once.  Measured on a B200
+// (graph replay): 16384 tokens of 32:8 FP16 heads of 128 62.5 us (344 MB, 5.5
+// TB/s), 24k tokens of 64:8 into the cache 161 us (971 MB, 6.0 TB/s), 4099 of
+// 32:32 FP32 heads of 64 21.6 us (135 MB, 6.2 TB/s); 64 tokens of 32:1 3.2 us
+// and 4 tokens into the cache 3.5 us, a launch and three trips to memory.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -362,7 +368,10 @@ struct StreamShape {
     size_t smem;
 };
 
-// Streaming kernel: tokens whose rows lie one after another (16-byte aligned).  A persistent CTA takes every gridDim-th token through a ring of
+// Streaming kernel: tokens whose rows lie one after another (16-byte aligned).
+// The bulk copies keep three stages per CTA in flight without registers (loads
+// into registers reached 2.8 TB/s), and three CTAs per SM of eight consumer warps
+// leave enough of them to hide the norm's exchanges (two CTAs 4.5 TB/s, four 5.0).  A persistent CTA takes every gridDim-th token through a ring of
 // stages: the producer warp brings a token's queries, keys, values and its
 // row of the rotation table by bulk copies, the consumer warps norm and rotate
 // the rows where they are, and the producer sends the whole token on by bulk

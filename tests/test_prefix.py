@@ -327,3 +327,16 @@ def test_refusals():
     dynamic = SharedPrefixPlan(layout, table, lengths, prefixes=members, max_lengths=lengths)
     with pytest.raises(ValueError):
         dynamic.run_dynamic(q, k, v, torch.tensor(table, device="cuda").long(), torch.tensor(lengths, device="cuda"))
+
+
+@pytest.mark.parametrize("batch,prompt,steps", [(3, 100, 20), (33, 1024, 5)])
+def test_the_example_runs(batch, prompt, steps):
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "paged-decode-lab_b200" / "examples" / "shared_prefix_loop.py"
+    spec = importlib.util.spec_from_file_location("shared_prefix_loop", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    result = module.run(batch=batch, prompt=prompt, steps=steps)
+    # values of the projection are about N(0, 1): the FP16 bounds above with |v| <= 6
+    assert result["shared_error"] < 6 * 2.0 ** -10 and result["apart_error"] < 6 * 2.0 ** -10
