@@ -51,7 +51,7 @@ struct SimtShape {
 // rows (32:8 heads of 128), shared memory reads and two barriers a step being the
 // rest; 16-row tiles (one query head per KV head) reach 15.
 template <int R, int D>
-__global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixArgs a) {
+__global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_constant__ PrefixArgs a) {
     using S = SimtShape<R, D>;
     constexpr int N = kSimtTokens, TR = R / 16, OR = R / 8, OD = D / 16;   // rows and dims of a thread's blocks
     extern __shared__ __align__(16) float sm[];
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const PrefixA
 // latency: 3 us for 1024 rows, 6 for 16384 of two pieces.
 constexpr int kMergeThreads = 256;
 template <typename Elt, int D>
-__global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const PrefixArgs a, int ways) {
+__global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __grid_constant__ PrefixArgs a, int ways) {
     constexpr int LANES = D / 8, BATCH = 4;
     __shared__ float sums[kMergeThreads][10];
     const int per_cta = kMergeThreads / LANES / ways;

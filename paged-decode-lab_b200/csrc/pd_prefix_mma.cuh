@@ -146,7 +146,7 @@ __device__ __forceinline__ RingCursor v_cursor(int t, bool paired) {
 template <int D, int T>
 __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     prefix_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const PrefixArgs a) {
+                      const __grid_constant__ PrefixArgs a) {
     using S = PrefixShape<D, T>;
     constexpr int NP = S::NP, SLOTS = S::SLOTS;
     extern __shared__ uint8_t smem_raw[];

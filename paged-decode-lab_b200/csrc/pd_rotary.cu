@@ -282,7 +282,7 @@ struct Lane {
 // row slots take rows slot, slot + slots, .. of [queries][keys][values], kRows of
 // them in flight before the token's place is looked up.
 template <typename Elt, int D, bool VECTOR, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
     using P = Part<Elt>;
     using L = Lane<Elt, D, INTERLEAVED>;
     constexpr int H = L::H, W = L::W, LANES = L::LANES;
@@ -377,7 +377,7 @@ struct StreamShape {
 // the rows where they are, and the producer sends the whole token on by bulk
 // stores.  Places are looked up by the producer's lanes, 32 tokens at a time.
 template <typename Elt, int D, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kStreamThreads, kStreamCtas) rotary_stream_kernel(const RotaryArgs a, const StreamShape sh) {
+__global__ void __launch_bounds__(kStreamThreads, kStreamCtas) rotary_stream_kernel(const __grid_constant__ RotaryArgs a, const __grid_constant__ StreamShape sh) {
     using L = Lane<Elt, D, INTERLEAVED>;
     constexpr int H = L::H, W = L::W, LANES = L::LANES, PER_WARP = L::PER_WARP;
     extern __shared__ __align__(128) uint8_t smem[];
