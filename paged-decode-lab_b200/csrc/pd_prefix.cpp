@@ -169,11 +169,11 @@ void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
                       std::max(shared_pages * page_bytes / 5e6, flops / (p.tile_rows == 16 ? 15e6 : 23e6));
         return;
     }
-    // Times in us (measured on a B200).  A CTA of the prefix kernel takes 7 for its start and end and
-    // 0.94 a step; the prefix's bytes come at 6.2e6 B/us at best.  The decode kernel takes 9 and its
+    // Estimated times in us, fitted to whole calls on a B200.  A CTA of the prefix kernel takes 7 steps
+    // for its start and end and 0.94 a step; the prefix's bytes come at 6.2e6 B/us at best.  The decode kernel takes 9 and its
     // bytes at 5.5e6 B/us, or 48e3 per SM, and 3 for each sequence on an SM.  The merge takes 3 and 350e3 FP32 values of partials a
     // us.  The two kernels run beside each other where both fit and that is sooner done.  (256
-    // sequences of 64:8 heads, 4096 shared and 512 own tokens each: 64 CTAs beside 84 136 us, 128 and then
+    // sequences of 64:8 heads, 4096 shared and 512 own tokens each: 64 CTAs beside 84 took 136 us, 128 and then
     // 148 174, 128 beside 20 364.)
     int64_t most = 1;
     for (const PrefixGroup &g : p.groups) most = std::max(most, steps_of(g));

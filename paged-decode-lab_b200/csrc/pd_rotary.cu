@@ -10,7 +10,8 @@
 //
 // Bound by memory: each head row is read and written once.  Measured on a B200
 // (graph replay): 16384 tokens of 32:8 FP16 heads of 128 62.5 us (344 MB, 5.5
-// TB/s), 24k tokens of 64:8 into the cache 161 us (971 MB, 6.0 TB/s), 4099 of
+// TB/s), 24k tokens of 64:8 into the cache 155 to 164 us (971 MB, 5.9 to 6.3
+// TB/s), 4099 of
 // 32:32 FP32 heads of 64 21.6 us (135 MB, 6.2 TB/s); 64 tokens of 32:1 3.2 us
 // and 4 tokens into the cache 3.5 us, a launch and three trips to memory.
 #include <algorithm>
