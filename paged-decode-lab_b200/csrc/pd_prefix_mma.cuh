@@ -426,9 +426,9 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 for (int e = 0; e < 16; ++e) {
                     const float2 z = unpack_f32x2(fma_f32x2(
                         pack_f32x2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, base2));
-                    const float w0 = ex2_approx(z.x), w1 = ex2_approx(z.y);
-                    sum = add_f32x2(sum, pack_f32x2(w0, w1));
-                    p[e] = pack_half2(w0, w1);
+                    p[e] = pack_half2(ex2_approx(z.x), ex2_approx(z.y));
+                    const float2 w = unpack_half2(p[e]);        // as the product sees them
+                    sum = add_f32x2(sum, pack_f32x2(w.x, w.y));
                 }
                 tc::st_32x32b_x16(block + 16 * c, p);
             };
