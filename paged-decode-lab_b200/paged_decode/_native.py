@@ -6,6 +6,7 @@ fails loudly when it is missing: there is no CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIB_NAME = "libpaged_decode_b200.so"
@@ -57,6 +58,9 @@ class Heads(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("out", ctypes.c_void_p), ("out_token_stride", ctypes.c_int64),
                 ("out_head_stride", ctypes.c_int64), ("heads", ctypes.c_int32)]
+
+
+pack_heads = struct.Struct("@PqqPqqi4x").pack    # Heads as bytes, for a call's own operands
 
 
 SIGNATURES = {

@@ -57,19 +57,20 @@ def _refuse_rows(x, name, shape, dtype, index):
     raise ValueError("inference only: detach tensors requiring gradients")
 
 
-def _fill(rows, x, out, name, shape, dtype, index):
-    """Check x (and out) [tokens, heads, head_dim] and describe them to the library."""
+def _heads(x, out, name, shape, dtype, index):
+    """Check x (and out) [tokens, heads, head_dim]; their pd_heads as bytes, each call's own (threads
+    may share the object; packing takes a fifth of the time of a ctypes structure)."""
     strides = x.stride()
     if x.shape != shape or x.dtype != dtype or x.get_device() != index or strides[2] != 1 or x.requires_grad:
         _refuse_rows(x, name, shape, dtype, index)
-    rows.data, rows.token_stride, rows.head_stride, rows.heads = x.data_ptr(), strides[0], strides[1], shape[1]
-    if out is not None:
-        if out is not x:
-            strides = out.stride()
-            if out.shape != shape or out.dtype != dtype or out.get_device() != index or strides[2] != 1 or \
-                    out.requires_grad:
-                _refuse_rows(out, f"{name}_out", shape, dtype, index)
-        rows.out, rows.out_token_stride, rows.out_head_stride = out.data_ptr(), strides[0], strides[1]
+    if out is None:
+        return _native.pack_heads(x.data_ptr(), strides[0], strides[1], 0, 0, 0, shape[1])
+    into = strides
+    if out is not x:
+        into = out.stride()
+        if out.shape != shape or out.dtype != dtype or out.get_device() != index or into[2] != 1 or out.requires_grad:
+            _refuse_rows(out, f"{name}_out", shape, dtype, index)
+    return _native.pack_heads(x.data_ptr(), strides[0], strides[1], out.data_ptr(), into[0], into[1], shape[1])
 
 
 def _int32(t, shape, name, index):
@@ -89,7 +90,8 @@ class HeadRotation:
     rotated, and None rotates nothing.  Pairs are (i, i + rotary_dim / 2), or
     with ``interleaved`` (2i, 2i + 1).  ``q_weight`` / ``k_weight`` [head_dim]
     norm the queries / keys before the rotation (None: no norm); they are kept
-    in FP32.  Everything is computed in FP32 and rounded once.
+    in FP32.  Everything is computed in FP32 and rounded once.  Threads and streams
+    may share an object: a call keeps nothing on it but the error word's flags.
     """
 
     def __init__(self, head_dim, table=None, *, interleaved=False, q_weight=None, k_weight=None, eps=1e-6,
@@ -124,8 +126,7 @@ class HeadRotation:
         self._error_at, self._index = self._error.data_ptr(), self.device.index
         self._spec = _native.Rotation(head_dim, self.rotary_dim, int(self.interleaved), self.eps, self.max_positions,
                                       *(None if t is None else t.data_ptr() for t in (table, *weights)))
-        self._rows = [_native.Heads(), _native.Heads()]
-        self._refs = (ctypes.addressof(self._spec), *map(ctypes.addressof, self._rows))
+        self._spec_at = ctypes.addressof(self._spec)
 
     def run(self, q, k, positions, *, q_out=None, k_out=None):
         """Returns (q_out, k_out): q [N, Hq, D] and k [N, Hkv, D] normed and rotated.
@@ -144,23 +145,22 @@ class HeadRotation:
             raise ValueError("heads must have shape [tokens, heads, head_dim]")
         dtype, index, tokens = first.dtype, self._index, first.shape[0]
         code = _dtype_code(dtype, "q/k")
-        outs, refs = [], []
-        for name, x, out, rows, ref in (("q", q, q_out, self._rows[0], self._refs[1]),
-                                        ("k", k, k_out, self._rows[1], self._refs[2])):
+        outs, descriptions = [], []
+        for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+            rows = None
             if x is None:
                 if out is not None:
                     raise ValueError(f"{name}_out without {name}")
-                ref = None
             else:
                 if x.ndim != 3:
                     raise ValueError("heads must have shape [tokens, heads, head_dim]")
                 if out is None:
                     out = torch.empty(x.shape, dtype=dtype, device=self.device)
-                _fill(rows, x, out, name, (tokens, x.shape[1], self.head_dim), dtype, index)
+                rows = _heads(x, out, name, (tokens, x.shape[1], self.head_dim), dtype, index)
             outs.append(out)
-            refs.append(ref)
+            descriptions.append(rows)
         status = self._lib.pd_rotate_heads(
-            self._refs[0], refs[0], refs[1], tokens, _int32(positions, (tokens,), "positions", index), code,
+            self._spec_at, *descriptions, tokens, _int32(positions, (tokens,), "positions", index), code,
             self._error_at, index, _native.stream_of(index))
         if status:
             _native.check(status, "rotate")
@@ -179,6 +179,7 @@ class CacheAppend:
 
     ``rotation`` (a ``HeadRotation``) norms and rotates keys, and queries given
     beside them, at their position in the sequence; None copies keys as they are.
+    Shared by threads and streams as a ``HeadRotation`` is.
     """
 
     def __init__(self, layout: Layout, rotation=None, *, device="cuda"):
@@ -199,9 +200,8 @@ class CacheAppend:
         self._layout = _native.Layout(layout.batch, layout.query_heads, layout.kv_heads, layout.head_dim,
                                       layout.page_size, layout.physical_pages)
         self._cache_shape = (layout.physical_pages, layout.page_size, layout.kv_heads, layout.head_dim)
-        self._rows = [_native.Heads(), _native.Heads(), _native.Heads()]
-        self._refs = (ctypes.addressof(self._layout), None if rotation is None else rotation._refs[0],
-                      *map(ctypes.addressof, self._rows))
+        self._layout_at = ctypes.addressof(self._layout)
+        self._spec_at = None if rotation is None else rotation._spec_at
 
     def run(self, k, v, k_cache, v_cache, table, lengths, *, q=None, indptr=None, q_out=None):
         """Write k, v [N, Hkv, D] into the caches; returns q's output (None without q).
@@ -223,17 +223,15 @@ class CacheAppend:
             raise ValueError("heads must have shape [tokens, heads, head_dim]")
         dtype, tokens, dim = k.dtype, k.shape[0], layout.head_dim
         code = _dtype_code(dtype, "k/v")
-        q_ref = None
+        q_rows = None
         if q is not None:
             if q_out is None:
                 q_out = torch.empty((tokens, layout.query_heads, dim), dtype=dtype, device=self.device)
-            _fill(self._rows[0], q, q_out, "q", (tokens, layout.query_heads, dim), dtype, index)
-            q_ref = self._refs[2]
+            q_rows = _heads(q, q_out, "q", (tokens, layout.query_heads, dim), dtype, index)
         elif q_out is not None:
             raise ValueError("q_out without q")
         shape = (tokens, layout.kv_heads, dim)
-        _fill(self._rows[1], k, None, "k", shape, dtype, index)
-        _fill(self._rows[2], v, None, "v", shape, dtype, index)
+        k_rows, v_rows = _heads(k, None, "k", shape, dtype, index), _heads(v, None, "v", shape, dtype, index)
         for cache in (k_cache, v_cache):
             if cache.shape != self._cache_shape or cache.dtype != dtype or cache.get_device() != index or \
                     not cache.is_contiguous() or cache.requires_grad:
@@ -248,7 +246,7 @@ class CacheAppend:
             raise ValueError("table must be a contiguous int32 CUDA tensor of shape [batch, width] on the device")
         width = table.shape[1]
         status = self._lib.pd_cache_append(
-            self._refs[0], self._refs[1], q_ref, self._refs[3], self._refs[4], tokens, k_cache.data_ptr(),
+            self._layout_at, self._spec_at, q_rows, k_rows, v_rows, tokens, k_cache.data_ptr(),
             v_cache.data_ptr(), code, _int32(table, (layout.batch, width), "table", index), width,
             _int32(lengths, (layout.batch,), "lengths", index), indptr_at, self._error_at, index,
             _native.stream_of(index))
