@@ -344,7 +344,8 @@ struct HalfEngine {
 
     // After reduce(): fold in another warp's reduced state for the same query heads,
     // o_s [heads][D] unnormalised and ml_s [heads] = (m, l), with the max-corrected
-    // merge (oracle.py:88-96); an empty state (l = 0) changes nothing.
+    // merge (oracle.py:88-96); an empty state (l = 0) changes nothing, and one whose
+    // l is NaN makes this one NaN (as everywhere below: only l = 0 counts as empty).
     __device__ __forceinline__ void absorb(const float *o_s, const float2 *ml_s) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -352,7 +353,7 @@ struct HalfEngine {
             for (int i = 0; i < 2; ++i) {
                 const int g = nt * 8 + 2 * (lane & 3) + i;
                 const float2 st = ml_s[g];
-                if (st.y > 0.f) {
+                if (st.y != 0.f) {
                     const float M = fmaxf(m[nt][i], st.x);
                     const float a = exp2f(m[nt][i] - M), b = exp2f(st.x - M);   // a = 0 for an empty state
                     m[nt][i] = M;
@@ -521,7 +522,7 @@ struct FloatEngine {
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
             const float2 st = ml_s[g];
-            if (st.y > 0.f) {
+            if (st.y != 0.f) {
                 const float M = fmaxf(m[g], st.x);
                 const float a = exp2f(m[g] - M), b = exp2f(st.x - M);
                 m[g] = M;
@@ -673,7 +674,7 @@ struct RowMerge {
     float4 o[CPL];
 
     __device__ __forceinline__ void add(float om, float ol, const float4 (&oo)[CPL]) {
-        if (!(ol > 0.f)) return;
+        if (ol == 0.f) return;
         const float nm = fmaxf(m, om);
         const float al = exp2f(m - nm), be = exp2f(om - nm);
         l = fmaf(l, al, be * ol);
@@ -739,7 +740,7 @@ struct RowMerge {
     __device__ __forceinline__ void write(const DecodeArgs &a, int4 meta, int lane, int xpar) const {
         const int c0 = LP > 1 ? lane % CH : lane;
         if (LP > 1 && lane >= CH) return;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = l != 0.f ? 1.f / l : 0.f;
         float4 v[CPL];
 #pragma unroll
         for (int cc = 0; cc < CPL; ++cc)
@@ -927,12 +928,12 @@ __device__ __forceinline__ void merge_ranks(const DecodeArgs &a, int warp, int l
         float top = -INFINITY;
 #pragma unroll
         for (int s = 0; s < kMaxRanks; ++s)
-            if (ml[s].y > 0.f) top = fmaxf(top, ml[s].x);
+            if (ml[s].y != 0.f) top = fmaxf(top, ml[s].x);
         float den = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int s = 0; s < kMaxRanks; ++s)
-            if (ml[s].y > 0.f) {
+            if (ml[s].y != 0.f) {
                 const float w = exp2f(ml[s].x - top) * ml[s].y;
                 den += w;
                 acc.x = fmaf(w, v[s].x, acc.x);
@@ -940,7 +941,7 @@ __device__ __forceinline__ void merge_ranks(const DecodeArgs &a, int warp, int l
                 acc.z = fmaf(w, v[s].z, acc.z);
                 acc.w = fmaf(w, v[s].w, acc.w);
             }
-        const float inv = den > 0.f ? 1.f / den : 0.f;
+        const float inv = den != 0.f ? 1.f / den : 0.f;
         if (lane < CH)
             reinterpret_cast<float4 *>(a.out + row * D)[lane] =
                 make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
@@ -1235,7 +1236,7 @@ __global__ void __launch_bounds__((HG * (GT / 8) * NSUB + 1) * 32, 1)
                 for (int x = 0; x < a.xworld; ++x) {
                     float *slot = xslot_of(a, x, xpar);
                     eng.for_each_o([&](int g, int d, float o, float, float l) {
-                        if (g < nw) slot[(qhead0 + g) * D + d] = l > 0.f ? o / l : 0.f;
+                        if (g < nw) slot[(qhead0 + g) * D + d] = l != 0.f ? o / l : 0.f;
                     });
                     eng.for_each_ml([&](int g, float m, float l) {
                         if (g < nw) *reinterpret_cast<float2 *>(xmeta_of<D>(slot, a, qhead0 + g)) = make_float2(m, l);
@@ -1245,7 +1246,7 @@ __global__ void __launch_bounds__((HG * (GT / 8) * NSUB + 1) * 32, 1)
             } else if (sg.w < 0) {
                 // the group's only segment, seen whole by this CTA: final output
                 eng.for_each_o([&](int g, int d, float o, float, float l) {
-                    if (g < nw) a.out[(qhead0 + g) * D + d] = l > 0.f ? o / l : 0.f;
+                    if (g < nw) a.out[(qhead0 + g) * D + d] = l != 0.f ? o / l : 0.f;
                 });
                 if (a.stats)
                     eng.for_each_ml([&](int g, float m, float l) {
@@ -1303,14 +1304,14 @@ __global__ void __launch_bounds__(kMergeThreads) merge_partials_kernel(const Dec
         float top = -INFINITY;
         for (int p = lane; p < parts; p += 32) {
             const float2 ml = a.part_ml[slot_row(p) * GT + g];
-            if (ml.y > 0.f) top = fmaxf(top, ml.x);
+            if (ml.y != 0.f) top = fmaxf(top, ml.x);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
         float den = 0.f;
         for (int p = lane; p < parts; p += 32) {
             const float2 ml = a.part_ml[slot_row(p) * GT + g];
-            if (ml.y > 0.f) den = fmaf(exp2f(ml.x - top), ml.y, den);
+            if (ml.y != 0.f) den = fmaf(exp2f(ml.x - top), ml.y, den);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(kFullMask, den, o);
@@ -1326,7 +1327,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_partials_kernel(const Dec
     for (int p = r; p < parts; p += lanes_p) {
         const int64_t pr = slot_row(p);
         const float2 ml = a.part_ml[pr * GT + g];
-        if (ml.y > 0.f) {
+        if (ml.y != 0.f) {
             const float w = exp2f(ml.x - top);
             const float4 o = reinterpret_cast<const float4 *>(a.part_o + (pr * GT + g) * D)[c];
             acc.x = fmaf(w, o.x, acc.x);
@@ -1347,7 +1348,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_partials_kernel(const Dec
         }
         const int64_t row = int64_t(g0.x) * a.Hq + int64_t(g0.y + hh) * a.group + g0.z + g;
         reinterpret_cast<float4 *>(a.out + row * D)[c] =
-            den > 0.f ? make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den)
+            den != 0.f ? make_float4(acc.x / den, acc.y / den, acc.z / den, acc.w / den)
                       : make_float4(0.f, 0.f, 0.f, 0.f);
         if (a.stats && c == 0) reinterpret_cast<float2 *>(a.stats)[row] = make_float2(top, den);
     }

@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(MqaShape<D, T>::THREADS, 1)
                 return true;
             }
             const int64_t qhead = int64_t(q.g0.x) * a.Hq + int64_t(q.g0.y) * a.group + q.g0.z + hrow;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float inv = l != 0.f ? 1.f / l : 0.f;
             if (q.sg.w < 0 && a.xworld) {
                 // the final row of this rank: to its slot in every rank's exchange buffer
                 for (int x = 0; x < a.xworld; ++x) {
@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(MqaShape<D, T>::THREADS, 1)
                 const float wo = mo.x == -INFINITY ? 0.f : ex2_ftz(mo.x - mx);
                 const float wp = mp.x == -INFINITY ? 0.f : ex2_ftz(mp.x - mx);
                 const float l = fmaf(mo.y, wo, mp.y * wp);
-                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const float inv = l != 0.f ? 1.f / l : 0.f;
                 const float so = wo * inv, sp = wp * inv;
                 const float *ro = reinterpret_cast<const float *>(pbuf) + r * D;
                 const float *rp = reinterpret_cast<const float *>(qbuf + S::Q_BYTES) + r * D;

@@ -5,7 +5,7 @@ namespace pd {
 
 // ------------------------------------------------------------------ cross-shard merge
 // out[row] = sum_s exp2(m_s - M) * l_s * o_s / sum_s exp2(m_s - M) * l_s over shards
-// with l_s > 0 (o_s is each shard's normalised output); zero when all are empty.
+// with l_s != 0 (o_s is each shard's normalised output); zero when all are empty.
 // Shard s's rows start at shard_out + s * stride and shard_stats + s * stride.
 static __global__ void merge_shards_kernel(const float *__restrict__ shard_out,
                                     const float *__restrict__ shard_stats, int shards, int64_t stride,
@@ -16,21 +16,21 @@ static __global__ void merge_shards_kernel(const float *__restrict__ shard_out,
     float top = -INFINITY;
     for (int s = 0; s < shards; ++s) {
         const float2 ml = *reinterpret_cast<const float2 *>(shard_stats + int64_t(s) * stride + 2 * row);
-        if (ml.y > 0.f) top = fmaxf(top, ml.x);
+        if (ml.y != 0.f) top = fmaxf(top, ml.x);
     }
     float den = 0.f;
     for (int s = 0; s < shards; ++s) {
         const float2 ml = *reinterpret_cast<const float2 *>(shard_stats + int64_t(s) * stride + 2 * row);
-        if (ml.y > 0.f) den = fmaf(exp2f(ml.x - top), ml.y, den);
+        if (ml.y != 0.f) den = fmaf(exp2f(ml.x - top), ml.y, den);
     }
     for (int d = lane; d < D; d += 32) {
         float num = 0.f;
         for (int s = 0; s < shards; ++s) {
             const float2 ml = *reinterpret_cast<const float2 *>(shard_stats + int64_t(s) * stride + 2 * row);
-            if (ml.y > 0.f)
+            if (ml.y != 0.f)
                 num = fmaf(exp2f(ml.x - top) * ml.y, shard_out[int64_t(s) * stride + row * D + d], num);
         }
-        out[row * D + d] = den > 0.f ? num / den : 0.f;
+        out[row * D + d] = den != 0.f ? num / den : 0.f;
     }
 }
 
