@@ -206,7 +206,8 @@ void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
     }
 }
 
-pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count) {
+pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, const int32_t *span,
+                            int32_t sm_count) {
     const pd_layout &L = p.layout;
     const int D = L.head_dim;
     const bool mma = p.dtype == PD_FLOAT16;
@@ -215,7 +216,10 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     const auto tiles_of = [&](const PrefixGroup &g) { return ceil_div(int64_t(g.members.size()) * p.group, p.tile_rows); };
     const auto steps_of = [&](const PrefixGroup &g) { return ceil_div(g.pages, step_pages); };
     p.seqs.assign(size_t(L.batch) * 8, 0);
-    for (int b = 0; b < L.batch; ++b) p.seqs[size_t(b) * 8] = -1;
+    for (int b = 0; b < L.batch; ++b) {
+        p.seqs[size_t(b) * 8] = -1;
+        p.seqs[size_t(b) * 8 + 5] = span[b];
+    }
     p.items.clear();
     p.tiles.clear();
     std::vector<int32_t> members, pages;

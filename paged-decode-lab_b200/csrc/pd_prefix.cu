@@ -220,6 +220,9 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __gri
         po += int64_t(tile.x) * a.tile_rows * D + lane * (a.tile_rows * 8) + row % a.tile_rows * 8;
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The decode kernel flags live lengths past the plan's; where it has nothing to do, this one does.
+    if (!a.rows && on && way == 0 && lane == 0 && __ldcg(a.lengths + b) > __ldg(a.seqs + 2 * b + 1).y)
+        atomicOr(a.error, PD_DEVERR_LENGTH);
     // a dynamic launch's sequence that ends inside its prefix
     if (prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size) {
         if (way == 0) row_inside<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, b, lane);
@@ -464,7 +467,7 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t wid
     s = create_suffix_plan(layout, table, width, lengths, max_lengths, first.data(), dtype, device, p.suffix_ctas,
                            &p.suffix);
     if (s != PD_OK) return s;
-    return build_prefix_plan(p, table, lengths, sm_count);
+    return build_prefix_plan(p, table, lengths, max_lengths ? max_lengths : lengths, sm_count);
 }
 
 }  // namespace

@@ -70,6 +70,8 @@ pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int
 void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count);
 
 // Lay the groups' work out and build the device image; the suffix plan is set.
-pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, int32_t sm_count);
+// span: the tokens that each sequence is planned for (max_lengths, or lengths).
+pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, const int32_t *span,
+                            int32_t sm_count);
 
 }  // namespace pd

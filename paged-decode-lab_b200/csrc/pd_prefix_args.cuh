@@ -18,7 +18,7 @@ struct PrefixArgs {
     // and per stream {row tile, first page, end page, slot}; kind kItem*.
     const int4 *items;
     // Per sequence: {member index in its group or -1, first row tile of KV head 0, row tiles per KV
-    // head, first of the group's pages in `pages`}, {shared pages, 0, 0, 0}.
+    // head, first of the group's pages in `pages`}, {shared pages, planned tokens, 0, 0}.
     const int4 *seqs;
     const int2 *tiles;          // per row tile: {first partial slot, pieces}
     const int32_t *members;     // sequences of the groups, one after another
