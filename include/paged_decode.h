@@ -447,8 +447,10 @@ pd_status pd_prefix_decode(pd_prefix_plan *plan, const void *q, const void *k, c
                            void *out, void *stream);
 
 /* One step of a dynamic plan with live metadata in device memory, as in
- * pd_decode_dynamic.  The shared pages are the plan's; a sequence whose live
- * length ends inside its prefix attends to its live tokens only. */
+ * pd_decode_dynamic: the live table and lengths count.  A sequence whose live
+ * table no longer starts with the plan's shared pages, or whose live length ends
+ * inside them, is computed on its own there (right, but slow: a plan is for tables
+ * that keep their prefixes). */
 pd_status pd_prefix_decode_dynamic(pd_prefix_plan *plan, const void *q, const void *k, const void *v,
                                    pd_dtype dtype, const int32_t *table, const int32_t *lengths, void *out,
                                    void *stream);

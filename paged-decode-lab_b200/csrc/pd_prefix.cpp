@@ -142,11 +142,12 @@ void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
     for (const PrefixGroup &g : p.groups) most_rows = std::max(most_rows, int64_t(g.members.size()) * p.group);
     p.tile_rows = int32_t(mma ? MmaShape::rows : most_rows > 16 ? 64 : 16);
     p.item_words = mma ? 16 : 8;
+    p.step_pages = int32_t((mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size);
     p.item_steps = 1;
     p.suffix_ctas = 0;
     p.shared_us = p.apart_us = 0;
     if (p.groups.empty()) return;
-    const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size;
+    const int64_t step_pages = p.step_pages;
     const auto tiles_of = [&](const PrefixGroup &g) { return ceil_div(int64_t(g.members.size()) * p.group, p.tile_rows); };
     const auto steps_of = [&](const PrefixGroup &g) { return ceil_div(g.pages, step_pages); };
     // What the decode kernel alone would take (us, measured on a B200): 12 and its bytes, the copies of
@@ -212,7 +213,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
     const int D = L.head_dim;
     const bool mma = p.dtype == PD_FLOAT16;
     const int64_t item_steps = p.item_steps;
-    const int64_t step_pages = (mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size;
+    const int64_t step_pages = p.step_pages;
     const auto tiles_of = [&](const PrefixGroup &g) { return ceil_div(int64_t(g.members.size()) * p.group, p.tile_rows); };
     const auto steps_of = [&](const PrefixGroup &g) { return ceil_div(g.pages, step_pages); };
     p.seqs.assign(size_t(L.batch) * 8, 0);
@@ -237,7 +238,7 @@ pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32
             s[4] = g.pages;
         }
         const int32_t m0 = int32_t(members.size()), n = int32_t(g.members.size()), pg = int32_t(pages.size());
-        // piece c of `pieces`: whole steps, as even as they come
+        // piece c of `pieces`: whole steps, as even as they come (prefix_merge_kernel has the same cut)
         const auto bound = [&](int64_t c, int64_t pieces) {
             return int32_t(std::min<int64_t>(g.pages, c * steps / pieces * step_pages));
         };

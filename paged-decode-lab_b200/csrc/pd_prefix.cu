@@ -50,7 +50,8 @@ struct SimtShape {
 // piece's end needs a mask.  Bound by the FMAs: 27 TFLOP/s of 74 on a B200 with 64
 // rows (32:8 heads of 128), shared memory reads and two barriers a step being the
 // rest; 16-row tiles (one query head per KV head) reach 15.
-template <int R, int D>
+// LIVE: a dynamic launch.
+template <int R, int D, bool LIVE>
 __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_constant__ PrefixArgs a) {
     using S = SimtShape<R, D>;
     constexpr int N = kSimtTokens, TR = R / 16, OR = R / 8, OD = D / 16;   // rows and dims of a thread's blocks
@@ -88,6 +89,15 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_
 #pragma unroll
         for (int k = 0; k < OD / 2; ++k) o[i][k] = 0;
     load(i1.y * T, 0);
+    // A dynamic launch: whether a row's live table has other pages in this piece.  kSimtThreads / R threads
+    // share a row's pages of each step, whose ids come while its scores are formed.
+    __shared__ int moved[R];
+    const int32_t *live_ids = nullptr;
+    if (LIVE) {
+        const int member = (i0.w * R + tid % R) / a.group;
+        if (member < i0.y) live_ids = a.table + __ldg(a.members + i0.x + member) * a.width;
+        if (tid < R) moved[tid] = 0;                    // (ordered by the barriers below)
+    }
     for (int t0 = i1.y * T, stage = 0; t0 < end; t0 += N, stage ^= 1) {
         if (t0 + N < end) {
             load(t0 + N, stage ^ 1);
@@ -96,6 +106,9 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         __syncthreads();
+        const int seen = t0 / T + tid / R;              // at most two pages a step, at least two threads a row
+        const bool looks = LIVE && live_ids && tid / R < N / T && seen < i1.z;
+        const int32_t id = looks ? __ldg(live_ids + seen) ^ __ldg(a.pages + i1.x + seen) : 0;
         // ---- scores
         const float *ks = sm + S::K + (stage * N + tg) * S::KS, *qs = sm + S::Q + rg * S::QS;
         f32x2 acc[TR][4];
@@ -139,6 +152,7 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_
             }
             if (tg == 0) sm[S::F + rg + 16 * i] = shrink;
         }
+        if (LIVE && id != 0) moved[tid % R] = 1;
         __syncthreads();
         // ---- output
         const float *vs = sm + S::V + stage * N * D + 4 * dg;
@@ -177,7 +191,10 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_
     for (int i = 0; i < TR; ++i) {
 #pragma unroll
         for (int x = 4; x > 0; x >>= 1) l[i] += __shfl_xor_sync(kFullMask, l[i], x);
-        if (tg == 0) a.part_ml[int64_t(i1.w) * R + rg + 16 * i] = make_float2(m[i], l[i]);
+        if (tg == 0) {
+            const bool usable = !LIVE || !moved[rg + 16 * i];
+            a.part_ml[int64_t(i1.w) * R + rg + 16 * i] = make_float2(m[i], usable ? l[i] : kPieceMoved);
+        }
     }
     float *po = a.part_o + int64_t(i1.w) * R * D;
 #pragma unroll
@@ -198,8 +215,9 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_
 // kernels in front are waited for; pieces are loaded four at a time.  Bound by
 // latency: 18 us for 16384 rows of head_dim 128 when profiled alone on cold caches.
 constexpr int kMergeThreads = 256;
-template <typename Elt, int D>
-__global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __grid_constant__ PrefixArgs a, int ways) {
+// LIVE: a dynamic launch.
+template <typename Elt, int D, bool LIVE>
+__global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __grid_constant__ PrefixArgs a, int ways) {
     constexpr int LANES = D / 8, BATCH = 4;
     __shared__ float sums[kMergeThreads][10];
     const int per_cta = kMergeThreads / LANES / ways;
@@ -223,16 +241,28 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __gri
     // The decode kernel flags live lengths past the plan's; where it has nothing to do, this one does.
     if (!a.rows && on && way == 0 && lane == 0 && __ldcg(a.lengths + b) > __ldg(a.seqs + 2 * b + 1).y)
         atomicOr(a.error, PD_DEVERR_LENGTH);
-    // a dynamic launch's sequence that ends inside its prefix
-    if (prefix_pages > 0 && __ldcg(a.lengths + b) < prefix_pages * a.page_size) {
-        if (way == 0) row_inside<Elt, D>(a, out_row, head / a.group, a.pages + sq.w, b, lane);
-        pieces = 0;
-        on = false;
+    // A dynamic launch's sequence that ends inside its prefix: computed on its own.
+    const int steps = (prefix_pages + a.step_pages - 1) / a.step_pages, count = pieces;
+    const auto start_of = [&](int p) {      // the first token of piece p, as the plan cuts them
+        return min(prefix_pages, p * steps / count * a.step_pages) * a.page_size;
+    };
+    int live = prefix_pages * a.page_size;
+    if (LIVE && count > 0) {
+        const int length = __ldcg(a.lengths + b);
+        if (length < live) {
+            live = length;
+            pieces = 0;
+        }
     }
+    bool moved = false;                     // a piece whose pages are others in the live table
     const int64_t ml_step = a.tile_rows, o_step = int64_t(a.tile_rows) * D;
     const float2 suffix = on && way == 0 ? suffix_stats(a, out_row) : make_float2(-INFINITY, 0.f);
     float top = top_of(suffix);
-    for (int p = way; p < pieces; p += ways) top = fmaxf(top, top_of(__ldcg(ml + p * ml_step)));
+    for (int p = way; p < pieces; p += ways) {
+        const float2 st = __ldcg(ml + p * ml_step);
+        if (LIVE && st.y == kPieceMoved) moved = true;
+        else top = fmaxf(top, top_of(st));
+    }
     RowSum sum(top);
     add_suffix<D>(sum, a, suffix, out_row, lane);
     for (int p0 = way; p0 < pieces; p0 += ways * BATCH) {
@@ -250,7 +280,21 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(const __gri
             }
         }
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j) sum.add(st[j], u[j], v[j]);
+        for (int j = 0; j < BATCH; ++j)
+            if (!LIVE || st[j].y != kPieceMoved) sum.add(st[j], u[j], v[j]);
+    }
+    if (LIVE && (moved || pieces < count)) {          // the other pieces, token by token
+        float o[8];
+        const int kv_head = head / a.group;
+        for (int p = way; p < pieces; p += ways)
+            if (__ldcg(ml + p * ml_step).y == kPieceMoved) {
+                const float2 st = walk<Elt, D>(a, out_row, kv_head, b, start_of(p), start_of(p + 1), kWalk, lane, o);
+                sum = joined(sum, st, o);
+            }
+        if (pieces < count && way == 0) {
+            const float2 st = walk<Elt, D>(a, out_row, kv_head, b, 0, live, kWalk, lane, o);
+            sum = joined(sum, st, o);
+        }
     }
     if (ways > 1) {
         float *mine = sums[threadIdx.x];
@@ -294,12 +338,13 @@ struct MmaEntry {
     size_t smem;
 };
 template <int D, int T>
-MmaEntry mma_entry() {
-    return {prefix_mma_kernel<D, T>, PrefixShape<D, T>::THREADS, PrefixShape<D, T>::SMEM};
+MmaEntry mma_entry(bool live) {
+    return {live ? prefix_mma_kernel<D, T, true> : prefix_mma_kernel<D, T, false>, PrefixShape<D, T>::THREADS,
+            PrefixShape<D, T>::SMEM};
 }
-MmaEntry mma_entry_for(const pd_layout &L) {
-    if (L.head_dim == 64) return L.page_size == 16 ? mma_entry<64, 16>() : mma_entry<64, 32>();
-    return L.page_size == 16 ? mma_entry<128, 16>() : mma_entry<128, 32>();
+MmaEntry mma_entry_for(const pd_layout &L, bool live) {
+    if (L.head_dim == 64) return L.page_size == 16 ? mma_entry<64, 16>(live) : mma_entry<64, 32>(live);
+    return L.page_size == 16 ? mma_entry<128, 16>(live) : mma_entry<128, 32>(live);
 }
 
 using SimtKernel = void (*)(const PrefixArgs);
@@ -307,35 +352,42 @@ struct SimtEntry {
     SimtKernel kernel;
     size_t smem;
 };
-template <int D>
-SimtEntry simt_entry(int rows) {
-    if (rows == 16) return {prefix_simt_kernel<16, D>, SimtShape<16, D>::FLOATS * 4};
-    return {prefix_simt_kernel<64, D>, SimtShape<64, D>::FLOATS * 4};
+template <int R, int D>
+SimtEntry simt_entry(bool live) {
+    return {live ? prefix_simt_kernel<R, D, true> : prefix_simt_kernel<R, D, false>, SimtShape<R, D>::FLOATS * 4};
+}
+SimtEntry simt_entry_for(const pd_prefix_plan &p, bool live) {
+    if (p.layout.head_dim == 64) return p.tile_rows == 16 ? simt_entry<16, 64>(live) : simt_entry<64, 64>(live);
+    return p.tile_rows == 16 ? simt_entry<16, 128>(live) : simt_entry<64, 128>(live);
 }
 
-// Allow the prefix kernel of this plan its shared memory.
+// Allow the prefix kernels of this plan their shared memory.
 cudaError_t allow_smem(const pd_prefix_plan &p) {
-    const void *kernel;
-    size_t smem;
-    if (p.dtype == PD_FLOAT16) {
-        const MmaEntry e = mma_entry_for(p.layout);
-        kernel = reinterpret_cast<const void *>(e.kernel), smem = e.smem;
-    } else {
-        const SimtEntry e = p.layout.head_dim == 64 ? simt_entry<64>(p.tile_rows) : simt_entry<128>(p.tile_rows);
-        kernel = reinterpret_cast<const void *>(e.kernel), smem = e.smem;
+    for (const bool live : {false, true}) {
+        if (live && !p.dynamic) break;
+        const void *kernel;
+        size_t smem;
+        if (p.dtype == PD_FLOAT16) {
+            const MmaEntry e = mma_entry_for(p.layout, live);
+            kernel = reinterpret_cast<const void *>(e.kernel), smem = e.smem;
+        } else {
+            const SimtEntry e = simt_entry_for(p, live);
+            kernel = reinterpret_cast<const void *>(e.kernel), smem = e.smem;
+        }
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (err != cudaSuccess) return err;
     }
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    return cudaSuccess;
 }
 
-template <int D>
 cudaError_t launch_prefix(const pd_prefix_plan &p, const PrefixArgs &a, const CUtensorMap &map_k,
                           const CUtensorMap &map_v, cudaStream_t stream) {
     const int64_t items = int64_t(p.items.size()) / p.item_words;
     if (p.dtype == PD_FLOAT16) {
-        const MmaEntry e = mma_entry_for(p.layout);
+        const MmaEntry e = mma_entry_for(p.layout, a.table != nullptr);
         return launch_dependent(e.kernel, items, e.threads, e.smem, stream, map_k, map_v, a);
     }
-    const SimtEntry e = simt_entry<D>(p.tile_rows);
+    const SimtEntry e = simt_entry_for(p, a.table != nullptr);
     return launch_dependent(e.kernel, items, kSimtThreads, e.smem, stream, a);
 }
 
@@ -343,9 +395,10 @@ template <int D>
 cudaError_t launch_merge(const pd_prefix_plan &p, const PrefixArgs &a, cudaStream_t stream) {
     const int64_t rows = int64_t(a.B) * a.Hq, per_cta = kMergeThreads / (D / 8) / p.merge_ways;
     const int64_t grid = (rows + per_cta - 1) / per_cta;
-    return p.dtype == PD_FLOAT16
-               ? launch_dependent(prefix_merge_kernel<__half, D>, grid, kMergeThreads, 0, stream, a, p.merge_ways)
-               : launch_dependent(prefix_merge_kernel<float, D>, grid, kMergeThreads, 0, stream, a, p.merge_ways);
+    const auto kernel = p.dtype == PD_FLOAT16
+                            ? (a.table ? prefix_merge_kernel<__half, D, true> : prefix_merge_kernel<__half, D, false>)
+                            : (a.table ? prefix_merge_kernel<float, D, true> : prefix_merge_kernel<float, D, false>);
+    return launch_dependent(kernel, grid, kMergeThreads, 0, stream, a, p.merge_ways);
 }
 
 pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const void *v, pd_dtype dtype,
@@ -373,6 +426,8 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.members = reinterpret_cast<const int32_t *>(p->dev + im.off_members);
     a.pages = reinterpret_cast<const int32_t *>(p->dev + im.off_pages);
     a.lengths = lengths ? lengths : reinterpret_cast<const int32_t *>(p->dev + im.off_lengths);
+    a.table = table;
+    a.width = p->width;
     a.part_o = reinterpret_cast<float *>(p->dev + im.off_part_o);
     a.part_ml = reinterpret_cast<float2 *>(p->dev + im.off_part_ml);
     a.out = out;
@@ -384,6 +439,7 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
     a.page_size = p->layout.page_size;
     a.tile_rows = p->tile_rows;
     a.P = p->layout.physical_pages;
+    a.step_pages = p->step_pages;
     a.scale_log2 = float(1.4426950408889634 / std::sqrt(double(p->layout.head_dim)));
     // The prefix kernel goes first: it lets the suffix's decode start beside it as soon as its own
     // CTAs have (FP16, on the SMs it leaves), and the merge waits for both.
@@ -394,7 +450,7 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
         alignas(64) CUtensorMap map_k, map_v;
         if (dtype == PD_FLOAT16) s = encode_prefix_maps(*p->suffix, k, v, &map_k, &map_v);
         if (s == PD_OK) {
-            err = wide ? launch_prefix<128>(*p, a, map_k, map_v, st) : launch_prefix<64>(*p, a, map_k, map_v, st);
+            err = launch_prefix(*p, a, map_k, map_v, st);
             if (err != cudaSuccess) s = fail(PD_ERR_CUDA, std::string("prefix launch: ") + cudaGetErrorString(err));
         }
     }

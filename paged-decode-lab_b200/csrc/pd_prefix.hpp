@@ -35,6 +35,7 @@ struct pd_prefix_plan {
     int32_t tile_rows = 0;          // query rows of one prefix tile
     int32_t slots = 0;              // partial slots (tile pieces)
     double shared_us = 0, apart_us = 0;   // estimates: with these groups, without any
+    int32_t step_pages = 0;         // pages of one step of the prefix kernel
     int64_t item_steps = 1;         // steps of the longest work item (choose_pieces)
     int32_t suffix_ctas = 0;        // SMs left to the suffix's decode beside the prefix kernel, 0: it runs behind it
     int32_t merge_ways = 1;         // thread sets that share a row's pieces in the merge

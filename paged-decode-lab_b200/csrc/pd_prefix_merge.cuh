@@ -3,40 +3,81 @@
 
 #include <cuda_fp16.h>
 
+#include "paged_decode.h"
 #include "pd_device.cuh"
 #include "pd_prefix_args.cuh"
 
 namespace pd {
 
-// (m, l) of one row over the first `limit` tokens of its prefix, and in `o`
-// eight dims of it: for a dynamic launch's sequence that ends inside its prefix,
-// whose row in the group's matrix covers the whole prefix.  D / 8 neighbouring
-// lanes, a token at a time: such lengths are rare, and most of them 0.
+// Eight elements of 16-byte aligned memory, in FP32.
+__device__ __forceinline__ void load8(float (&x)[8], const float *src) {
+    const float4 u = __ldcg(reinterpret_cast<const float4 *>(src)), v = __ldcg(reinterpret_cast<const float4 *>(src) + 1);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+}
+__device__ __forceinline__ void load8(float (&x)[8], const __half *src) {
+    const uint4 u = __ldcg(reinterpret_cast<const uint4 *>(src));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack_half2(w[i]);
+        x[2 * i] = v.x, x[2 * i + 1] = v.y;
+    }
+}
+
+// (m, l) of one row over tokens from .. to of sequence b's live table, kWalk of every `step`
+// (from: the start of kWalk tokens of a page), and in `o` eight dims of it: for a dynamic
+// launch's pieces that the group's matrix does not describe.  D / 8 neighbouring lanes.  Tokens of pages
+// outside the cache are skipped and flagged, as in the decode kernel.
+constexpr int kWalk = 4;
 template <typename Elt, int D>
-__device__ __forceinline__ float2 prefix_row(const PrefixArgs &a, int64_t row, int kv_head, const int32_t *pages,
-                                          int limit, int lane, float (&o)[8]) {
+__device__ __noinline__ float2 walk(const PrefixArgs &a, int64_t row, int kv_head, int b, int from, int to, int step,
+                                    int lane, float (&o)[8]) {
     constexpr int LANES = D / 8;
     const unsigned mates = ((1u << LANES) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
+    const int32_t *pages = a.table + b * a.width;
     float q[8], m = -INFINITY, l = 0.f;
+    load8(q, static_cast<const Elt *>(a.q) + row * D + lane * 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        q[i] = float(static_cast<const Elt *>(a.q)[row * D + lane * 8 + i]) * a.scale_log2;
-        o[i] = 0.f;
-    }
-    for (int t = 0; t < limit; ++t) {
-        const int64_t at = ((int64_t(pages[t / a.page_size]) * a.page_size + t % a.page_size) * a.Hkv + kv_head) * D +
-                           lane * 8;
-        float s = 0.f;
+    for (int i = 0; i < 8; ++i) q[i] *= a.scale_log2, o[i] = 0.f;
+    for (int t = from; t < to; t += step) {
+        const int64_t page = __ldcg(pages + t / a.page_size);
+        if (page < 0 || page >= a.P) {
+            if (lane == 0) atomicOr(a.error, PD_DEVERR_BAD_PAGE);
+            continue;
+        }
+        const int64_t at = ((page * a.page_size + t % a.page_size) * a.Hkv + kv_head) * D + lane * 8;
+        const int64_t row_step = int64_t(a.Hkv) * D;
+        float s[kWalk], top = m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(q[i], float(static_cast<const Elt *>(a.k)[at + i]), s);
+        for (int j = 0; j < kWalk; ++j) {           // (the rest of a page is there, whatever it holds)
+            float x[8];
+            load8(x, static_cast<const Elt *>(a.k) + at + j * row_step);
+            s[j] = 0.f;
 #pragma unroll
-        for (int x = LANES / 2; x > 0; x >>= 1) s += __shfl_xor_sync(mates, s, x);
-        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-        const float shrink = exp2f(m - base), p = exp2f(s - base);
-        l = fmaf(l, shrink, p);
+            for (int i = 0; i < 8; ++i) s[j] = fmaf(q[i], x[i], s[j]);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmaf(o[i], shrink, p * float(static_cast<const Elt *>(a.v)[at + i]));
+        for (int j = 0; j < kWalk; ++j) {
+#pragma unroll
+            for (int x = LANES / 2; x > 0; x >>= 1) s[j] += __shfl_xor_sync(mates, s[j], x);
+            if (t + j >= to) s[j] = -INFINITY;
+            top = fmaxf(top, s[j]);
+        }
+        const float base = top == -INFINITY ? 0.f : top, shrink = exp2f(m - base);
         m = top;
+        l *= shrink;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] *= shrink;
+#pragma unroll
+        for (int j = 0; j < kWalk; ++j) {
+            if (t + j >= to) break;
+            float x[8];
+            load8(x, static_cast<const Elt *>(a.v) + at + j * row_step);
+            const float p = exp2f(s[j] - base);
+            l += p;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = fmaf(p, x[i], o[i]);
+        }
     }
     return make_float2(m, l);
 }
@@ -73,6 +114,14 @@ struct RowSum {
 // What counts for the maximum.
 __device__ __forceinline__ float top_of(float2 ml) { return ml.y != 0.f ? ml.x : -INFINITY; }
 
+// Two parts' sum, each with a maximum of its own.
+__device__ __forceinline__ RowSum joined(const RowSum &x, float2 ml, const float (&o)[8]) {
+    RowSum sum(fmaxf(top_of(make_float2(x.top, x.den)), top_of(ml)));
+    sum.add(make_float2(x.top, x.den), x.o);
+    sum.add(ml, o);
+    return sum;
+}
+
 // The suffix decode's (m, l) of a row, and its normalised row as a part.
 __device__ __forceinline__ float2 suffix_stats(const PrefixArgs &a, int64_t row) {
     return a.rows ? __ldcg(reinterpret_cast<const float2 *>(a.stats) + row) : make_float2(-INFINITY, 0.f);
@@ -92,19 +141,6 @@ __device__ __forceinline__ void store_row(RowSum &sum, const PrefixArgs &a, int6
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum.o[i] *= inv;
     store8(static_cast<Elt *>(a.out) + row * D + lane * 8, sum.o);
-}
-
-// The whole row of a sequence that ends inside its prefix (a dynamic launch).
-template <typename Elt, int D>
-__device__ __noinline__ void row_inside(const PrefixArgs &a, int64_t row, int kv_head, const int32_t *pages, int b,
-                                        int lane) {
-    float o[8];
-    const float2 ml = prefix_row<Elt, D>(a, row, kv_head, pages, __ldcg(a.lengths + b), lane, o);
-    const float2 suffix = suffix_stats(a, row);
-    RowSum sum(fmaxf(top_of(ml), top_of(suffix)));
-    add_suffix<D>(sum, a, suffix, row, lane);
-    sum.add(ml, o);
-    store_row<Elt, D>(sum, a, row, lane);
 }
 
 }  // namespace pd

@@ -27,7 +27,7 @@
 // 2^7 below the step's maximum, so weights stay within (0, 2^15] and FP16 keeps
 // its full precision down to 2^-21 of the largest.  The denominator sums the
 // FP32 weights.  Rows are either in use for the whole prefix or their results
-// are dropped (a live length inside the prefix: the merge kernel's slow path),
+// are dropped (a live length inside the prefix, or other pages there: the merge kernel's slow path),
 // so no scores need masks; a last step of fewer pages takes fewer columns.
 //
 // Each stream leaves its rows' (m, l, o) as a partial for the merge kernel.  The
@@ -69,7 +69,7 @@ struct PrefixShape {
     static constexpr int S_COL = 0, O_COL = 4 * NS;
     static constexpr int TMEM_COLS = 512;
     static constexpr int NBARS = 2 * SLOTS + 2 + 4 + 4 + 2 + 2 + 1;
-    static constexpr size_t SMEM = 1024 + 2 * size_t(Q_BYTES) + size_t(SLOTS) * STEP_BYTES + NBARS * 8 + 16;
+    static constexpr size_t SMEM = 1024 + 2 * size_t(Q_BYTES) + size_t(SLOTS) * STEP_BYTES + NBARS * 8 + 16 + 2 * M * 4;
     static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory budget");
     static_assert(SMEM <= 232448 && SMEM > 116 * 1024, "one CTA per SM: tensor memory is never contended");
 };
@@ -143,7 +143,8 @@ __device__ __forceinline__ RingCursor v_cursor(int t, bool paired) {
     return RingCursor{first, paired ? 2 * S::V_SLOTS : S::V_SLOTS, first, 0};
 }
 
-template <int D, int T>
+// LIVE: a dynamic launch.
+template <int D, int T, bool LIVE>
 __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     prefix_mma_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const __grid_constant__ PrefixArgs a) {
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
     uint64_t *mma_done = o_last + 2;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(mma_done + 1);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1) + 1;
+    int *moved = reinterpret_cast<int *>(mma_done + 1) + 4;     // [stream][a member's first row of the tile]
 
     const int warp = int(__reduce_max_sync(kFullMask, threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const PrefixItem it = prefix_item(a, blockIdx.x);
@@ -194,6 +196,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         tc::relinquish_alloc_permit();
         tc::fence_before_sync();
     }
+    if (LIVE && threadIdx.x < 2 * S::M) moved[threadIdx.x] = 0;
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
@@ -356,6 +359,18 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(q_full + t));
         }
+        // A dynamic launch: whether the live table of the row's member has other pages in this run.  The threads of
+        // a member's rows share the pages of each step, whose ids come while its scores do.
+        const int row = st.tile * S::M + r, member = row / a.group;
+        const int first_row = max(0, member * a.group - st.tile * S::M);
+        const int32_t *live_ids = nullptr, *planned_ids = a.pages + it.page0 + st.first;
+        unsigned mine = 0;                              // this thread's pages of a step
+        bool other = false;
+        if (LIVE && member < it.members && n > 0) {
+            const int mates = min(S::M, (member + 1) * a.group - st.tile * S::M) - first_row;
+            live_ids = a.table + __ldg(a.members + it.member0 + member) * a.width + st.first;
+            for (int p = r - first_row; p < NP; p += mates) mine |= 1u << p;
+        }
         const uint32_t lanes = uint32_t(32 * quad) << 16;
         const uint32_t ts = tmem + lanes + S::S_COL + 2 * t * S::NS, to = tmem + lanes + S::O_COL + t * D;
         const auto warp_wait = [&](uint64_t *bar, int parity) {
@@ -365,6 +380,13 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         unsigned long long l2 = 0, l3 = 0;              // four partial denominators
         bool ok = true;
         for (int i = 0; i < n; ++i) {
+            int32_t ids[NP];                            // the difference to the planned ones
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int at = i * NP + p;
+                const bool on = LIVE && (mine >> p & 1) && at < st.end - st.first;
+                ids[p] = on ? __ldg(live_ids + at) ^ __ldg(planned_ids + at) : 0;
+            }
             if (!warp_wait(s_full + 2 * t + (i & 1), i >> 1 & 1)) {
                 ok = false;
                 break;
@@ -438,6 +460,12 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * t + (i & 1)));
+#pragma unroll
+            for (int p = 0; p < NP; ++p) other = other || ids[p] != 0;
+        }
+        if (LIVE) {
+            if (other) moved[t * S::M + first_row] = 1;
+            named_barrier_sync(1 + t, S::M);
         }
         if (!ok && lane == 0) fail_wait();
         // ------------------------------------------------------------ the row's part
@@ -448,7 +476,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         }
         tc::fence_after_sync();
         const float2 l = unpack_f32x2(add_f32x2(l2, l3));
-        const bool on = n > 0 && ok && (st.tile * S::M + r) / a.group < it.members;
+        const bool on = n > 0 && ok && member < it.members;
         if (n > 0) {
             // partials lie [D / 8][rows][8]: a row's reads take whole sectors, as do a thread's stores
             float *dst = a.part_o + (int64_t(st.slot) * D * S::M + r * 8);
@@ -462,7 +490,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                     store_sector(dst + (c / 8 + 1) * (S::M * 8), o + 8);
                 }
             }
-            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, l.x + l.y);
+            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, LIVE && moved[t * S::M + first_row] ? kPieceMoved : l.x + l.y);
         }
         tc::fence_before_sync();
     }

@@ -177,9 +177,11 @@ class SharedPrefixPlan:
     def run_dynamic(self, q, k, v, table, lengths, out=None):
         """Decode with live metadata in device memory (plans built with ``max_lengths``).
 
-        As ``DecodePlan.run_dynamic``.  The shared pages are the plan's; a
-        sequence whose live length ends inside its prefix (0: not in use)
-        attends to its live tokens only.
+        As ``DecodePlan.run_dynamic``: the live table and lengths count.  A
+        sequence whose live table no longer starts with the plan's shared
+        pages, or whose live length ends inside them (0: not in use), is
+        computed on its own there: right, but slow, so build a new plan when
+        prefixes change.
         """
         if self.max_lengths is None:
             raise ValueError("run_dynamic needs a plan built with max_lengths")

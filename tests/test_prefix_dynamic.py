@@ -48,3 +48,99 @@ def test_a_length_past_a_plan_that_ends_with_its_prefixes_is_flagged(dtype, othe
         assert plan.read_errors() == _native.PD_DEVERR_LENGTH
         assert torch.equal(out, want)
     assert torch.equal(plan.run_dynamic(q, k, v, cuda(table), cuda(lengths)), want) and plan.read_errors() == 0
+
+
+def exact(q, k, v, table, lengths):
+    """Attention in 64 bits and the weights' average of |v|; tokens on pages outside the cache are left out."""
+    B, H, D = q.shape
+    P, page, kv = k.shape[:3]
+    out, size = (torch.zeros((B, H, D), dtype=torch.float64) for _ in range(2))
+    for b, n in enumerate(int(x) for x in lengths):
+        at = np.arange(n)
+        ids = np.asarray(table)[b, at // page].astype(np.int64)
+        slots = torch.tensor((ids * page + at % page)[(ids >= 0) & (ids < P)], device="cuda")
+        if len(slots) == 0:
+            continue
+        kk, vv = (x.flatten(0, 1)[slots].double().transpose(0, 1) for x in (k, v))
+        w = torch.softmax(q[b].double().view(kv, -1, D) @ kk.mT / D ** 0.5, -1)
+        out[b], size[b] = (w @ vv).view(H, D).cpu(), (w @ vv.abs()).view(H, D).cpu()
+    return out, size
+
+
+def close(got, want, size):
+    """FP16: weights rounded to 2^-11 of themselves in numerator and denominator, one rounding at the store;
+    scores and sums are FP32."""
+    tol = 2e-5 * (size + want.abs()) + 1e-6
+    if got.dtype == F16:
+        tol = tol + 2.0 ** -11 * (1.05 * size + 2.1 * want.abs()) + 2.0 ** -24
+    worst = ((got.cpu().double() - want).abs() - tol).max().item()
+    assert worst <= 0, f"{worst:.3g} over the tolerance"     # NaN fails too
+
+
+def serving_batch(sharers, shared, others, heads, kv, D, page, dtype, own=3, spare=60):
+    """Sequences behind `shared` common pages with room for `own` pages more, others apart, and spare pages."""
+    rng = np.random.default_rng(11)
+    batch = sharers + others
+    pages = shared + (batch * own + others * shared) + spare
+    pool = list(rng.permutation(pages))
+    common = [pool.pop() for _ in range(shared)]
+    table = np.zeros((batch, shared + own), dtype=np.int32)
+    for b in range(batch):
+        head = common if b < sharers else [pool.pop() for _ in range(shared)]
+        table[b] = head + [pool.pop() for _ in range(own)]
+    lengths = (shared * page + rng.integers(0, own * page + 1, batch)).astype(np.int32)
+    layout = Layout(batch, heads, kv, D, page, pages)
+    return layout, table, lengths, np.array(pool, dtype=np.int32), *tensors(layout, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("heads,kv,D,page", [(32, 8, 128, 16), (6, 6, 64, 32), (1, 1, 64, 16), (32, 1, 128, 32)])
+def test_pages_that_move_under_a_plan(dtype, heads, kv, D, page):
+    """The live table counts, as in DecodePlan.run_dynamic, also where a sequence no longer starts with the
+    plan's shared pages: a page copied elsewhere, another sequence in the slot, a page outside the cache."""
+    shared, sharers = 9, 12
+    layout, table, lengths, spare, q, k, v = serving_batch(sharers, shared, 3, heads, kv, D, page, dtype)
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=[(range(sharers), shared)], dtype=dtype,
+                            max_lengths=np.full(layout.batch, table.shape[1] * page))
+
+    def run(live_table, live, flags=0):
+        out = plan.run_dynamic(q, k, v, cuda(live_table), cuda(live))
+        close(out, *exact(q, k, v, live_table, live))
+        assert plan.read_errors() == flags
+        return out.clone()
+
+    before = run(table, lengths)
+    for moved in ([0], [shared - 1], [4], [2, 7], list(range(shared))):
+        live = table.copy()
+        live[5, moved] = spare[: len(moved)]
+        after = run(live, lengths)
+        same = [b for b in range(layout.batch) if b != 5]
+        assert torch.equal(after[same], before[same]) and not torch.equal(after[5], before[5])
+    slot = table.copy()                              # other sequences in two slots, one longer, one shorter
+    slot[3], slot[8] = spare[:shared + 3], spare[12:12 + shared + 3]
+    live = lengths.copy()
+    live[3], live[8], live[1], live[2] = table.shape[1] * page, 2 * page + 5, 0, shared * page
+    run(slot, live)
+    slot[1] = -1                                     # not in use: its row may hold anything
+    run(slot, live)
+    everyone = table.copy()                          # the whole group behind another prefix
+    everyone[:sharers, :shared] = spare[20:20 + shared]
+    run(everyone, lengths)
+    for bad in (-1, layout.physical_pages, np.iinfo(np.int32).max):
+        broken = table.copy()
+        broken[4, 3] = bad
+        run(broken, lengths, _native.PD_DEVERR_BAD_PAGE)
+    assert torch.equal(run(table, lengths), before)
+
+
+def test_found_groups_follow_the_live_table_too():
+    """The caller named no groups: a slot that another sequence took over still gets its own attention."""
+    sharers, shared, page = 48, 128, 16
+    layout, table, lengths, spare, q, k, v = serving_batch(sharers, shared, 0, 32, 8, 128, page, F16, spare=200)
+    plan = SharedPrefixPlan(layout, table, lengths, max_lengths=lengths)
+    assert len(plan.prefixes) == 1
+    live = table.copy()
+    live[7, :shared + 3] = spare[: shared + 3]
+    out = plan.run_dynamic(q, k, v, cuda(live), cuda(lengths))
+    close(out, *exact(q, k, v, live, lengths))
+    assert plan.read_errors() == 0
