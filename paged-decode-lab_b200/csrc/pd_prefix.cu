@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
     // The decode kernel flags live lengths past the plan's; where it has nothing to do, this one does.
     if (!a.rows && on && way == 0 && lane == 0 && __ldcg(a.lengths + b) > __ldg(a.seqs + 2 * b + 1).y)
         atomicOr(a.error, PD_DEVERR_LENGTH);
-    // A dynamic launch's sequence that ends inside its prefix: computed on its own.
+    // A dynamic launch's sequence that ends inside its prefix: pieces before its end count.
     const int steps = (prefix_pages + a.step_pages - 1) / a.step_pages, count = pieces;
     const auto start_of = [&](int p) {      // the first token of piece p, as the plan cuts them
         return min(prefix_pages, p * steps / count * a.step_pages) * a.page_size;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
         const int length = __ldcg(a.lengths + b);
         if (length < live) {
             live = length;
-            pieces = 0;
+            while (pieces > 0 && start_of(pieces) > live) --pieces;
         }
     }
     bool moved = false;                     // a piece whose pages are others in the live table
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
         for (int j = 0; j < BATCH; ++j)
             if (!LIVE || st[j].y != kPieceMoved) sum.add(st[j], u[j], v[j]);
     }
-    if (LIVE && (moved || pieces < count)) {          // the other pieces, token by token
+    if (LIVE && (moved || pieces < count)) {    // the other pieces, token by token
         float o[8];
         const int kv_head = head / a.group;
         for (int p = way; p < pieces; p += ways)
@@ -291,8 +291,9 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
                 const float2 st = walk<Elt, D>(a, out_row, kv_head, b, start_of(p), start_of(p + 1), kWalk, lane, o);
                 sum = joined(sum, st, o);
             }
-        if (pieces < count && way == 0) {
-            const float2 st = walk<Elt, D>(a, out_row, kv_head, b, 0, live, kWalk, lane, o);
+        if (pieces < count) {               // the piece that the sequence ends in: all sets
+            const float2 st = walk<Elt, D>(a, out_row, kv_head, b, start_of(pieces) + way * kWalk, live, kWalk * ways,
+                                           lane, o);
             sum = joined(sum, st, o);
         }
     }

@@ -144,3 +144,47 @@ def test_found_groups_follow_the_live_table_too():
     out = plan.run_dynamic(q, k, v, cuda(live), cuda(lengths))
     close(out, *exact(q, k, v, live, lengths))
     assert plan.read_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("sharers,shared", [(6, 700), (40, 70)])
+def test_lengths_at_every_cut_of_a_prefix(dtype, sharers, shared):
+    """Live lengths around the ends of pieces, steps and pages, a sequence each."""
+    page = 16
+    layout, table, lengths, _, q, k, v = serving_batch(sharers, shared, 1, 8, 2, 64, page, dtype)
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=[(range(sharers), shared)], dtype=dtype,
+                            max_lengths=np.full(layout.batch, table.shape[1] * page))
+    rng = np.random.default_rng(5)
+    for _ in range(6):
+        live = lengths.copy()
+        cuts = rng.integers(0, shared + 1, sharers) * page + rng.choice([-17, -3, -1, 0, 1, 5, 15], sharers)
+        live[:sharers] = np.clip(cuts, 0, table.shape[1] * page)
+        moved = table.copy()
+        moved[rng.integers(0, sharers), rng.integers(0, shared)] = table[sharers, 0]       # and a page that moved
+        out = plan.run_dynamic(q, k, v, cuda(moved), cuda(live))
+        close(out, *exact(q, k, v, moved, live))
+        assert plan.read_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_a_length_inside_a_long_prefix_costs_a_piece_of_it(dtype):
+    """One sequence a token short of 49152: the pieces before its last one serve it too.  (Token by token over
+    the whole prefix the step took more than a hundred times as long as planned.)"""
+    page, shared = 32, 1536
+    layout, table, lengths, _, q, k, v = serving_batch(8, shared, 0, 32, 8, 128, page, dtype)
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=[(range(8), shared)], dtype=dtype, max_lengths=lengths)
+    short = lengths.copy()
+    short[2] = shared * page - 1
+    times = {}
+    for name, live in (("planned", cuda(lengths)), ("short", cuda(short))):
+        live_table, begin, end = cuda(table), *(torch.cuda.Event(enable_timing=True) for _ in range(2))
+        plan.run_dynamic(q, k, v, live_table, live)
+        times[name] = 1e9
+        for _ in range(5):
+            begin.record()
+            out = plan.run_dynamic(q, k, v, live_table, live)
+            end.record()
+            end.synchronize()
+            times[name] = min(times[name], begin.elapsed_time(end))
+    close(out[2:3], *exact(q[2:3], k, v, table[2:3], short[2:3]))
+    assert times["short"] < 25 * times["planned"], times
