@@ -52,7 +52,8 @@ typedef enum pd_dtype { PD_FLOAT16 = 0, PD_FLOAT32 = 1 } pd_dtype;
 #define PD_DEVERR_TIMEOUT 1u      /* a bounded wait on a shared-memory barrier ran out */
 #define PD_DEVERR_BAD_PAGE 2u     /* a live page id outside [0, physical_pages): tokens skipped */
 #define PD_DEVERR_LENGTH 8u       /* a dynamic launch's length exceeded the plan's max_lengths: clamped;
-                                     an append's token lies outside its page table row: skipped */
+                                     an append's token lies outside its page table row
+                                     or in no sequence's range: skipped */
 #define PD_DEVERR_POSITION 16u    /* a position outside the rotation table: the token is skipped */
 
 /* Replaces oracle.Layout (src/paged_decode/oracle.py:11-27). */
@@ -375,9 +376,9 @@ pd_status pd_rotate_heads(const pd_rotation *rotation, const pd_heads *q, const 
  * are normed and rotated (rotation may be NULL: copied) at their position in
  * the sequence, values are copied bit for bit; q (may be NULL) is normed and
  * rotated into q.out.  Padding and skipped tokens write no cache row and
- * leave zero query rows; a token outside its table row or the rotation table,
- * or on a page outside the cache, is skipped and flags PD_DEVERR_LENGTH,
- * PD_DEVERR_POSITION or PD_DEVERR_BAD_PAGE in *error.  k.out and v.out are not
+ * leave zero query rows; a token before indptr[0] or outside its table row, outside
+ * the rotation table, or on a page outside the cache is skipped and flags
+ * PD_DEVERR_LENGTH, PD_DEVERR_POSITION or PD_DEVERR_BAD_PAGE in *error.  k.out and v.out are not
  * used.  Two tokens must not share a slot.  Asynchronous, allocation-free,
  * one launch. */
 pd_status pd_cache_append(const pd_layout *layout, const pd_rotation *rotation, const pd_heads *q,

@@ -143,7 +143,9 @@ __device__ __forceinline__ Place place_of(const RotaryArgs &a, int64_t token, bo
     if constexpr (APPEND) {
         int b;
         int64_t to_end;     // tokens from this one to the sequence's end
+        bool before = false;                            // of the first sequence's range
         if (a.indptr) {
+            before = token < __ldg(a.indptr);
             b = sequence_of(a.indptr, a.batch, token);
             to_end = __ldg(a.indptr + b + 1) - token;   // <= 0: padding past the last sequence
         } else {
@@ -154,7 +156,7 @@ __device__ __forceinline__ Place place_of(const RotaryArgs &a, int64_t token, bo
         p.position = length - to_end;
         if (to_end <= 0 || (!a.indptr && length == 0)) {
             p.live = false;                             // padding, or a sequence that is not in use
-        } else if (p.position < 0 || p.position >= (a.width << a.page_shift)) {
+        } else if (before || p.position < 0 || p.position >= (a.width << a.page_shift)) {
             flag = kErrLength;
         } else {
             const int at = int(p.position);

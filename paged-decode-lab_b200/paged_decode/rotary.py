@@ -209,7 +209,7 @@ class CacheAppend:
         ``lengths`` int32 [B] already count the new tokens and ``table`` int32
         [B, W] already names their pages: both are what ``run_dynamic`` takes
         next.  With ``indptr`` int32 [B + 1] tokens indptr[b] .. indptr[b+1] - 1
-        are the last ones of sequence b (tokens from indptr[B] on are padding);
+        are the last ones of sequence b (indptr[0] is 0, tokens from indptr[B] on are padding);
         without it token b is the last one of sequence b, and a sequence of
         length 0 is not in use.  q [N, Hq, D] is normed and rotated into
         ``q_out`` (default: a new tensor; q itself: in place).  Padding and
