@@ -127,6 +127,7 @@ class HeadRotation:
         self._spec = _native.Rotation(head_dim, self.rotary_dim, int(self.interleaved), self.eps, self.max_positions,
                                       *(None if t is None else t.data_ptr() for t in (table, *weights)))
         self._spec_at = ctypes.addressof(self._spec)
+        torch.cuda.current_stream(self.device).synchronize()    # a call may come on any stream
 
     def run(self, q, k, positions, *, q_out=None, k_out=None):
         """Returns (q_out, k_out): q [N, Hq, D] and k [N, Hkv, D] normed and rotated.
@@ -202,6 +203,7 @@ class CacheAppend:
         self._cache_shape = (layout.physical_pages, layout.page_size, layout.kv_heads, layout.head_dim)
         self._layout_at = ctypes.addressof(self._layout)
         self._spec_at = None if rotation is None else rotation._spec_at
+        torch.cuda.current_stream(self.device).synchronize()
 
     def run(self, k, v, k_cache, v_cache, table, lengths, *, q=None, indptr=None, q_out=None):
         """Write k, v [N, Hkv, D] into the caches; returns q's output (None without q).
