@@ -30,6 +30,7 @@ def _native_plan(layout, table, lengths, prefixes, max_lengths, code, device_ind
         max_lengths = np.ascontiguousarray(max_lengths, dtype=np.int32)
     count, arrays = find, [None, None, None]
     if prefixes is not None:
+        prefixes = list(prefixes)
         members = [np.asarray(m) for m, _ in prefixes]
         if any(m.ndim != 1 or (m.size and m.dtype.kind not in "iu") for m in members):
             raise TypeError("prefixes must be pairs (sequence indices, pages)")

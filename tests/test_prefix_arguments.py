@@ -1,0 +1,26 @@
+"""What the Python side hands to the prefix plan builder (no GPU)."""
+import numpy as np
+import pytest
+
+from paged_decode.layout import Layout
+from paged_decode.prefix import inspect_prefix_plan
+
+LAYOUT = Layout(5, 8, 2, 64, 16, 40)
+TABLE = np.array([[0, 1, 2, 9, 10], [0, 1, 2, 11, 12], [3, 4, 13, 14, 15], [3, 4, 16, 17, 18], [0, 1, 2, 19, 20]])
+LENGTHS = np.array([70, 80, 33, 60, 49])
+GROUPS = [([0, 1, 4], 3), ([2, 3], 2)]
+
+
+def described(prefixes, **kw):
+    info, groups, items = inspect_prefix_plan(LAYOUT, TABLE, LENGTHS, prefixes=prefixes, **kw)
+    return info, [(m.tolist(), p) for m, p in groups], items.tolist()
+
+
+def test_prefixes_from_any_iterable():
+    """The list is walked more than once."""
+    want = described(GROUPS)
+    assert want[1] == GROUPS
+    assert described(iter(GROUPS)) == want
+    assert described((m, p) for m, p in GROUPS) == want
+    assert described(zip([m for m, _ in GROUPS], [p for _, p in GROUPS])) == want
+    assert described((tuple(m), np.int32(p)) for m, p in GROUPS) == want
