@@ -9,6 +9,7 @@ meet by their softmax statistics.
 from __future__ import annotations
 
 import ctypes
+from numbers import Integral
 
 import numpy as np
 
@@ -32,7 +33,8 @@ def _native_plan(layout, table, lengths, prefixes, max_lengths, code, device_ind
     if prefixes is not None:
         prefixes = list(prefixes)
         members = [np.asarray(m) for m, _ in prefixes]
-        if any(m.ndim != 1 or (m.size and m.dtype.kind not in "iu") for m in members):
+        if any(m.ndim != 1 or (m.size and m.dtype.kind not in "iu") for m in members) or \
+                any(isinstance(p, bool) or not isinstance(p, Integral) for _, p in prefixes):
             raise TypeError("prefixes must be pairs (sequence indices, pages)")
         sizes = [m.size for m in members]
         if any(((m < 0) | (m >= layout.batch)).any() for m in members):

@@ -24,3 +24,10 @@ def test_prefixes_from_any_iterable():
     assert described((m, p) for m, p in GROUPS) == want
     assert described(zip([m for m, _ in GROUPS], [p for _, p in GROUPS])) == want
     assert described((tuple(m), np.int32(p)) for m, p in GROUPS) == want
+
+
+@pytest.mark.parametrize("pages", [2.7, 2.0, True, "2", None, np.float32(1), 2 + 0j])
+def test_page_counts_are_integers(pages):
+    """As members are: nothing is truncated."""
+    with pytest.raises(TypeError, match="sequence indices, pages"):
+        described([([0, 1], pages)])
