@@ -63,6 +63,15 @@ def _groups(lib, handle, batch):
     return info, [(np.flatnonzero(group == g), int(pages[g])) for g in range(info.groups)]
 
 
+def _check_max_lengths(max_lengths, layout, table, lengths):
+    max_lengths = np.asarray(max_lengths)
+    if max_lengths.shape != lengths.shape or max_lengths.dtype.kind not in "iu":
+        raise ValueError("max_lengths must be integers of shape [batch]")
+    if (max_lengths < lengths).any() or (max_lengths > table.shape[1] * layout.page_size).any():
+        raise ValueError("max_lengths must lie between lengths and the page table capacity")
+    return max_lengths
+
+
 def find_prefixes(layout: Layout, table, lengths, *, dtype="float16"):
     """The groups of sequences that start with the same pages, [(sequence indices, pages)].
 
@@ -85,6 +94,8 @@ def inspect_prefix_plan(layout: Layout, table, lengths, *, prefixes=None, dtype=
     """A host-only plan's (info, groups, work items) as pd_prefix_plan_copy_items lays them out (no GPU needed)."""
     _check_limits(layout, 256, "serial")
     table, lengths = validate_metadata(layout, table, lengths)
+    if max_lengths is not None:
+        max_lengths = _check_max_lengths(max_lengths, layout, table, lengths)
     lib = _native.load()
     code = {"float16": _native.PD_FLOAT16, "float32": _native.PD_FLOAT32}[dtype]
     handle = _native_plan(layout, table, lengths, prefixes, max_lengths, code, -1)
@@ -119,11 +130,7 @@ class SharedPrefixPlan:
         _check_limits(layout, 256, "serial")
         table, lengths = validate_metadata(layout, table, lengths)
         if max_lengths is not None:
-            max_lengths = np.asarray(max_lengths)
-            if max_lengths.shape != lengths.shape or max_lengths.dtype.kind not in "iu":
-                raise ValueError("max_lengths must be integers of shape [batch]")
-            if (max_lengths < lengths).any() or (max_lengths > table.shape[1] * layout.page_size).any():
-                raise ValueError("max_lengths must lie between lengths and the page table capacity")
+            max_lengths = _check_max_lengths(max_lengths, layout, table, lengths)
         self.layout, self.dtype, self.max_lengths = layout, dtype, max_lengths
         self.device = _cuda_device(device)
         self._lib = _native.load()

@@ -31,3 +31,12 @@ def test_page_counts_are_integers(pages):
     """As members are: nothing is truncated."""
     with pytest.raises(TypeError, match="sequence indices, pages"):
         described([([0, 1], pages)])
+
+
+def test_inspected_plans_check_max_lengths_as_plans_do():
+    """Too few or misshapen ones do not reach the library, which reads one per sequence."""
+    for bad in (LENGTHS[:3], LENGTHS[None], LENGTHS + 0.5, np.array(80), LENGTHS - 1, LENGTHS + 80,
+                np.array([2 ** 32 + 80] * 5)):
+        with pytest.raises(ValueError, match="max_lengths"):
+            described(GROUPS, max_lengths=bad)
+    assert described(GROUPS, max_lengths=[80, 80, 80, 80, 80])[0]["dynamic"] == 1
