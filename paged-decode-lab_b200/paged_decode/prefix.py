@@ -9,7 +9,7 @@ meet by their softmax statistics.
 from __future__ import annotations
 
 import ctypes
-from numbers import Integral
+import operator
 
 import numpy as np
 
@@ -33,13 +33,18 @@ def _native_plan(layout, table, lengths, prefixes, max_lengths, code, device_ind
     if prefixes is not None:
         prefixes = list(prefixes)
         members = [np.asarray(m) for m, _ in prefixes]
-        if any(m.ndim != 1 or (m.size and m.dtype.kind not in "iu") for m in members) or \
-                any(isinstance(p, bool) or not isinstance(p, Integral) for _, p in prefixes):
-            raise TypeError("prefixes must be pairs (sequence indices, pages)")
+        pages = [p for _, p in prefixes]
+        try:
+            if any(isinstance(p, bool) for p in pages):
+                raise TypeError
+            pages = np.asarray([operator.index(p) for p in pages], dtype=np.int64)
+            if any(m.ndim != 1 or (m.size and m.dtype.kind not in "iu") for m in members):
+                raise TypeError
+        except TypeError:
+            raise TypeError("prefixes must be pairs (sequence indices, pages)") from None
         sizes = [m.size for m in members]
         if any(((m < 0) | (m >= layout.batch)).any() for m in members):
             raise ValueError("prefix group names a sequence outside the batch")
-        pages = np.asarray([p for _, p in prefixes], dtype=np.int64).reshape(-1)
         if ((pages < 1) | (pages > table.shape[1])).any():
             raise ValueError("a prefix must have 1 .. table width pages")
         count = len(sizes)

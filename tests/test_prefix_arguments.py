@@ -40,3 +40,8 @@ def test_inspected_plans_check_max_lengths_as_plans_do():
         with pytest.raises(ValueError, match="max_lengths"):
             described(GROUPS, max_lengths=bad)
     assert described(GROUPS, max_lengths=[80, 80, 80, 80, 80])[0]["dynamic"] == 1
+
+
+@pytest.mark.parametrize("three", [np.array(3), np.int64(3), np.uint8(3)])
+def test_page_counts_of_any_integer_kind(three):
+    assert described([([0, 1], three)])[1] == [([0, 1], 3)]
