@@ -68,6 +68,14 @@ def _groups(lib, handle, batch):
     return info, [(np.flatnonzero(group == g), int(pages[g])) for g in range(info.groups)]
 
 
+def _named_dtype_code(dtype):
+    """The library's code of "float16" or torch.float16, .. (torch need not be there)."""
+    code = {"float16": _native.PD_FLOAT16, "float32": _native.PD_FLOAT32}.get(str(dtype).removeprefix("torch."))
+    if code is None:
+        raise TypeError("dtype must be float16 or float32")
+    return code
+
+
 def _check_max_lengths(max_lengths, layout, table, lengths):
     max_lengths = np.asarray(max_lengths)
     if max_lengths.shape != lengths.shape or max_lengths.dtype.kind not in "iu":
@@ -87,7 +95,7 @@ def find_prefixes(layout: Layout, table, lengths, *, dtype="float16"):
     _check_limits(layout, 256, "serial")
     table, lengths = validate_metadata(layout, table, lengths)
     lib = _native.load()
-    code = {"float16": _native.PD_FLOAT16, "float32": _native.PD_FLOAT32}[dtype]
+    code = _named_dtype_code(dtype)
     handle = _native_plan(layout, table, lengths, None, None, code, -1, find=-2)
     try:
         return _groups(lib, handle, layout.batch)[1]
@@ -102,7 +110,7 @@ def inspect_prefix_plan(layout: Layout, table, lengths, *, prefixes=None, dtype=
     if max_lengths is not None:
         max_lengths = _check_max_lengths(max_lengths, layout, table, lengths)
     lib = _native.load()
-    code = {"float16": _native.PD_FLOAT16, "float32": _native.PD_FLOAT32}[dtype]
+    code = _named_dtype_code(dtype)
     handle = _native_plan(layout, table, lengths, prefixes, max_lengths, code, -1)
     try:
         info, groups = _groups(lib, handle, layout.batch)

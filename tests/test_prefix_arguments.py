@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from paged_decode.layout import Layout
-from paged_decode.prefix import inspect_prefix_plan
+from paged_decode.prefix import find_prefixes, inspect_prefix_plan
 
 LAYOUT = Layout(5, 8, 2, 64, 16, 40)
 TABLE = np.array([[0, 1, 2, 9, 10], [0, 1, 2, 11, 12], [3, 4, 13, 14, 15], [3, 4, 16, 17, 18], [0, 1, 2, 19, 20]])
@@ -45,3 +45,14 @@ def test_inspected_plans_check_max_lengths_as_plans_do():
 @pytest.mark.parametrize("three", [np.array(3), np.int64(3), np.uint8(3)])
 def test_page_counts_of_any_integer_kind(three):
     assert described([([0, 1], three)])[1] == [([0, 1], 3)]
+
+
+def test_types_by_name_or_as_torch_has_them():
+    torch = pytest.importorskip("torch")
+    for name in ("float16", "float32"):
+        want = described(GROUPS, dtype=name)
+        assert described(GROUPS, dtype=getattr(torch, name)) == want
+        assert [(m.tolist(), p) for m, p in find_prefixes(LAYOUT, TABLE, LENGTHS, dtype=getattr(torch, name))] == GROUPS
+    for bad in ("bfloat16", torch.bfloat16, None):
+        with pytest.raises(TypeError, match="float16 or float32"):
+            find_prefixes(LAYOUT, TABLE, LENGTHS, dtype=bad)
