@@ -414,8 +414,8 @@ typedef struct pd_prefix_info {
  * g has members[indptr[g]] .. members[indptr[g + 1] - 1] (sequences, each in
  * at most one group) sharing their first pages[g] pages, all of them whole
  * (lengths >= pages * page_size) and equal in the table.  group_count -2 finds
- * the groups in the table, -1 uses the found ones only if they save enough
- * (otherwise none).
+ * the groups in the table, -1 uses those of the found ones that save enough
+ * (all, some or none).
  * max_lengths (NULL: a static plan) as in pd_plan_create_dynamic.  device < 0
  * builds a host-only plan. */
 pd_status pd_prefix_plan_create(const pd_layout *layout, const int32_t *table, int64_t table_width,

@@ -8,7 +8,10 @@
 
 #include <algorithm>
 #include <cstring>
+#include <map>
 #include <numeric>
+#include <set>
+#include <utility>
 
 namespace pd {
 
@@ -132,79 +135,157 @@ struct MmaShape {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-}  // namespace
+// Groups of one shape: `count` of them, each with so many members and shared pages.
+struct GroupShape {
+    int64_t members, pages, count;
+    int64_t saved() const { return (members - 1) * pages; }
+};
 
-void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
+// The shapes of some groups, those of which one saves the most first.
+std::vector<GroupShape> shapes_of(const std::vector<PrefixGroup> &groups) {
+    std::map<std::pair<int64_t, int64_t>, int64_t> counts;
+    for (const PrefixGroup &g : groups) ++counts[{int64_t(g.members.size()), int64_t(g.pages)}];
+    std::vector<GroupShape> shapes;
+    for (const auto &c : counts) shapes.push_back({c.first.first, c.first.second, c.second});
+    std::stable_sort(shapes.begin(), shapes.end(), [](const GroupShape &a, const GroupShape &b) { return a.saved() > b.saved(); });
+    return shapes;
+}
+
+struct PrefixCut {
+    double us = 0;                  // estimated time of a call
+    int64_t item_steps = 1;
+    int32_t suffix_ctas = 0;
+};
+
+int32_t tile_rows_for(bool mma, int64_t most_rows) { return int32_t(mma ? MmaShape::rows : most_rows > 16 ? 64 : 16); }
+
+// The decode kernel reads copies of pages that others read too from L2 (B/us, measured on a B200).
+double copy_rate(const pd_prefix_plan &p) { return p.dtype != PD_FLOAT16 ? 9e6 : p.group > 16 ? 7.5e6 : 14e6; }
+
+double page_bytes_of(const pd_prefix_plan &p) {
+    return (p.dtype == PD_FLOAT16 ? 4.0 : 8.0) * p.layout.page_size * p.layout.kv_heads * p.layout.head_dim;
+}
+
+// How these groups' work is best cut, and what a call then takes; the decode kernel has
+// suffix_pages beside them, and `copies` reads of pages that it could have shared.
+PrefixCut cut_of(const pd_prefix_plan &p, const std::vector<GroupShape> &shapes, int64_t suffix_pages, int64_t copies,
+                 int32_t sm_count) {
     const pd_layout &L = p.layout;
     const bool mma = p.dtype == PD_FLOAT16;
-    p.group = L.query_heads / L.kv_heads;
-    int64_t most_rows = 0;
-    for (const PrefixGroup &g : p.groups) most_rows = std::max(most_rows, int64_t(g.members.size()) * p.group);
-    p.tile_rows = int32_t(mma ? MmaShape::rows : most_rows > 16 ? 64 : 16);
-    p.item_words = mma ? 16 : 8;
-    p.step_pages = int32_t((mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / L.page_size);
-    p.item_steps = 1;
-    p.suffix_ctas = 0;
-    p.shared_us = p.apart_us = 0;
-    if (p.groups.empty()) return;
-    const int64_t step_pages = p.step_pages;
-    const auto tiles_of = [&](const PrefixGroup &g) { return ceil_div(int64_t(g.members.size()) * p.group, p.tile_rows); };
-    const auto steps_of = [&](const PrefixGroup &g) { return ceil_div(g.pages, step_pages); };
-    // What the decode kernel alone would take (us, measured on a B200): 12 and its bytes, the copies of
-    // shared pages from L2.
-    const double page_bytes = (mma ? 4.0 : 8.0) * L.page_size * L.kv_heads * L.head_dim;
-    int64_t copies = 0, shared_pages = 0;
-    double flops = 0;
-    for (const PrefixGroup &g : p.groups) {
-        copies += int64_t(g.members.size()) * g.pages;
-        shared_pages += g.pages;
-        flops += 4.0 * L.kv_heads * double(tiles_of(g) * p.tile_rows) * g.pages * L.page_size * L.head_dim;
+    const double page_bytes = page_bytes_of(p);
+    int64_t most_rows = 0, shared_pages = 0;
+    for (const GroupShape &g : shapes) {
+        most_rows = std::max(most_rows, g.members * p.group);
+        shared_pages += g.count * g.pages;
     }
-    p.apart_us = 12 + suffix_pages * page_bytes / 5.5e6 +
-                 copies * page_bytes / (!mma ? 9e6 : p.group > 16 ? 7.5e6 : 14e6);
+    const int64_t rows = tile_rows_for(mma, most_rows);
+    const auto tiles_of = [&](const GroupShape &g) { return ceil_div(g.members * p.group, rows); };
+    const auto steps_of = [&](const GroupShape &g) { return ceil_div(g.pages, p.step_pages); };
+    PrefixCut cut;
     if (!mma) {
         int64_t work = 0;
-        for (const PrefixGroup &g : p.groups) work += L.kv_heads * tiles_of(g) * steps_of(g);
-        p.item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, (p.tile_rows == 16 ? 4 : 2) * sm_count));
-        p.shared_us = 22 + suffix_pages * page_bytes / 5.5e6 +
-                      std::max(shared_pages * page_bytes / 5e6, flops / (p.tile_rows == 16 ? 15e6 : 23e6));
-        return;
+        double flops = 0;
+        for (const GroupShape &g : shapes) {
+            work += g.count * L.kv_heads * tiles_of(g) * steps_of(g);
+            flops += 4.0 * L.kv_heads * double(g.count * tiles_of(g) * rows) * g.pages * L.page_size * L.head_dim;
+        }
+        cut.item_steps = std::max<int64_t>(1, work / std::max<int64_t>(1, (rows == 16 ? 4 : 2) * sm_count));
+        cut.us = 22 + suffix_pages * page_bytes / 5.5e6 + copies * page_bytes / copy_rate(p) +
+                 std::max(shared_pages * page_bytes / 5e6, flops / (rows == 16 ? 15e6 : 23e6));
+        return cut;
     }
     // Estimated times in us, fitted to whole calls on a B200.  A CTA of the prefix kernel takes 7 steps
-    // for its start and end and 0.94 a step; the prefix's bytes come at 6.2e6 B/us at best.  The decode kernel takes 9 and its
-    // bytes at 5.5e6 B/us, or 48e3 per SM, and 3 for each sequence on an SM.  The merge takes 3 and 350e3 FP32 values of partials a
-    // us.  The two kernels run beside each other where both fit and that is sooner done.  (256
-    // sequences of 64:8 heads, 4096 shared and 512 own tokens each: 64 CTAs beside 84 took 136 us, 128 and then
-    // 148 174, 128 beside 20 364.)
-    int64_t most = 1;
-    for (const PrefixGroup &g : p.groups) most = std::max(most, steps_of(g));
+    // for its start and end and 0.94 a step; the prefix's bytes come at 6.2e6 B/us at best.  The decode kernel
+    // takes 9 and its bytes at 5.5e6 B/us, or 48e3 per SM, and 3 for each sequence on an SM.  The merge takes
+    // 3 and 350e3 FP32 values of partials a us.  The two kernels run beside each other where both fit and that is
+    // sooner done.  (256 sequences of 64:8 heads, 4096 shared and 512 own tokens each: 64 CTAs beside 84 took
+    // 136 us, 128 and then 148 174, 128 beside 20 364.)
     const double segments = double(L.batch) * ceil_div(L.kv_heads, 8) * ceil_div(p.group, 32);
     const auto suffix_us = [&](int64_t sms) {
-        return suffix_pages == 0
-                   ? 0.0
-                   : 9 + suffix_pages * page_bytes / std::min(5.5e6, 48e3 * double(sms)) + 3 * segments / double(sms);
+        if (suffix_pages + copies == 0) return 0.0;
+        return 9 + suffix_pages * page_bytes / std::min(5.5e6, 48e3 * double(sms)) +
+               copies * page_bytes / (copy_rate(p) * double(sms) / sm_count) + 3 * segments / double(sms);
     };
-    double best = 1e300;
-    for (int64_t steps = 1; steps <= most; ++steps) {
-        int64_t ctas = 0, values = 0;
-        for (const PrefixGroup &g : p.groups) {
-            const int64_t tiles = tiles_of(g), pieces = ceil_div(steps_of(g), steps);
-            ctas += L.kv_heads * (tiles / 2 * pieces + tiles % 2 * ceil_div(pieces, 2));
-            values += L.query_heads * int64_t(g.members.size()) * L.head_dim * pieces;
+    // the shortest item for every number of pieces of the first (largest) few shapes
+    std::set<int64_t> lengths;
+    for (size_t i = 0; i < std::min<size_t>(shapes.size(), 8); ++i)
+        for (int64_t steps = 1, all = steps_of(shapes[i]); steps <= all;) {
+            lengths.insert(steps);
+            const int64_t pieces = ceil_div(all, steps);
+            if (pieces == 1) break;
+            steps = ceil_div(all, pieces - 1);
         }
-        const double prefix = std::max(0.94 * double(ceil_div(ctas, sm_count) * (7 + steps)),
+    cut.us = 1e300;
+    for (const int64_t steps : lengths) {
+        int64_t ctas = 0, total = 0, longest = 0, values = 0;      // total, longest: in steps
+        for (const GroupShape &g : shapes) {
+            const int64_t tiles = tiles_of(g), pieces = ceil_div(steps_of(g), steps);
+            const int64_t own = L.kv_heads * g.count * (tiles / 2 * pieces + tiles % 2 * ceil_div(pieces, 2));
+            const int64_t length = 7 + ceil_div(steps_of(g), pieces);
+            ctas += own;
+            total += own * length;
+            longest = std::max(longest, length);
+            values += L.query_heads * g.count * g.members * L.head_dim * pieces;
+        }
+        // waves of CTAs of the mean length, but no less than the longest
+        const double prefix = std::max(0.94 * std::max(double(longest), double(ceil_div(ctas, sm_count)) * total / ctas),
                                        7 + shared_pages * page_bytes / 6.2e6);
         const double behind = prefix + suffix_us(sm_count);
-        const double beside =
-            suffix_pages > 0 && ctas < sm_count ? std::max(prefix, suffix_us(sm_count - ctas)) : behind;
-        const double us = std::min(beside, behind) + 3 + double(values) / 350e3;
-        if (us < best) {
-            best = us;
-            p.shared_us = us + 4;
-            p.item_steps = steps;
-            p.suffix_ctas = beside < behind ? int32_t(sm_count - ctas) : 0;
-        }
+        const double beside = suffix_pages + copies > 0 && ctas < sm_count ? std::max(prefix, suffix_us(sm_count - ctas))
+                                                                           : behind;
+        const double us = 4 + std::min(beside, behind) + 3 + double(values) / 350e3;
+        if (us < cut.us) cut = PrefixCut{us, steps, beside < behind ? int32_t(sm_count - ctas) : 0};
     }
+    return cut;
+}
+
+}  // namespace
+
+void keep_paying_groups(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
+    const std::vector<GroupShape> shapes = shapes_of(p.groups);
+    int64_t copies = 0;             // of the shapes that are not used
+    for (const GroupShape &g : shapes) copies += g.count * g.members * g.pages;
+    // without any: the decode kernel alone, 12 us and its bytes
+    const double page_bytes = page_bytes_of(p);
+    double best = 12 + suffix_pages * page_bytes / 5.5e6 + copies * page_bytes / copy_rate(p);
+    size_t kept = 0;
+    // the first k shapes, for at most some 64 values of k
+    std::vector<GroupShape> used;
+    const size_t stride = std::max<size_t>(1, shapes.size() / 64);
+    for (size_t k = 1; k <= shapes.size(); ++k) {
+        const GroupShape &g = shapes[k - 1];
+        used.push_back(g);
+        copies -= g.count * g.members * g.pages;
+        if (k > 16 && k % stride && k < shapes.size()) continue;
+        const double us = cut_of(p, used, suffix_pages, copies, sm_count).us;
+        if (us < best) best = us, kept = k;
+    }
+    std::set<std::pair<int64_t, int64_t>> keep;
+    for (size_t k = 0; k < kept; ++k) keep.insert({shapes[k].members, shapes[k].pages});
+    p.groups.erase(std::remove_if(p.groups.begin(), p.groups.end(),
+                                  [&](const PrefixGroup &g) {
+                                      return !keep.count({int64_t(g.members.size()), int64_t(g.pages)});
+                                  }),
+                   p.groups.end());
+}
+
+void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count) {
+    int64_t most_rows = 0;
+    for (const PrefixGroup &g : p.groups) most_rows = std::max(most_rows, int64_t(g.members.size()) * p.group);
+    p.tile_rows = tile_rows_for(p.dtype == PD_FLOAT16, most_rows);
+    p.item_steps = 1;
+    p.suffix_ctas = 0;
+    if (p.groups.empty()) return;
+    const PrefixCut cut = cut_of(p, shapes_of(p.groups), suffix_pages, 0, sm_count);
+    p.item_steps = cut.item_steps;
+    p.suffix_ctas = cut.suffix_ctas;
+}
+
+void set_shape(pd_prefix_plan &p) {
+    const bool mma = p.dtype == PD_FLOAT16;
+    p.group = p.layout.query_heads / p.layout.kv_heads;
+    p.item_words = mma ? 16 : 8;
+    p.step_pages = int32_t((mma ? MmaShape::step_tokens : SimtPlan::step_tokens) / p.layout.page_size);
 }
 
 pd_status build_prefix_plan(pd_prefix_plan &p, const int32_t *table, const int32_t *lengths, const int32_t *span,

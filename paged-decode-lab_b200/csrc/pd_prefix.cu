@@ -505,22 +505,21 @@ pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t wid
         if (err != cudaSuccess) return fail(PD_ERR_CUDA, std::string("device query: ") + cudaGetErrorString(err));
     }
     std::vector<int32_t> first(layout->batch, 0);
-    const auto choose = [&]() {
+    const int32_t *span = max_lengths ? max_lengths : lengths;
+    const auto suffix_pages = [&]() {       // the pages outside of all groups
         std::fill(first.begin(), first.end(), 0);
         for (const PrefixGroup &g : p.groups)
             for (const int32_t b : g.members) first[b] = g.pages;
-        const int32_t *span = max_lengths ? max_lengths : lengths;
-        int64_t suffix_pages = 0;
+        int64_t pages = 0;
         for (int b = 0; b < layout->batch; ++b)
-            suffix_pages += std::max<int64_t>(0, (int64_t(span[b]) + layout->page_size - 1) / layout->page_size - first[b]);
-        p.suffix_empty = suffix_pages == 0;
-        choose_pieces(p, suffix_pages, sm_count);
+            pages += std::max<int64_t>(0, (int64_t(span[b]) + layout->page_size - 1) / layout->page_size - first[b]);
+        return pages;
     };
-    choose();
-    if (group_count == -1 && p.shared_us >= p.apart_us) {   // sharing would not pay
-        p.groups.clear();
-        choose();
-    }
+    set_shape(p);
+    if (group_count == -1) keep_paying_groups(p, suffix_pages(), sm_count);
+    const int64_t rest = suffix_pages();
+    p.suffix_empty = rest == 0;
+    choose_pieces(p, rest, sm_count);
     s = create_suffix_plan(layout, table, width, lengths, max_lengths, first.data(), dtype, device, p.suffix_ctas,
                            &p.suffix);
     if (s != PD_OK) return s;

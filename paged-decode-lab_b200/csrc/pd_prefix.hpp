@@ -34,7 +34,6 @@ struct pd_prefix_plan {
     int32_t group = 0;              // G = Hq / Hkv
     int32_t tile_rows = 0;          // query rows of one prefix tile
     int32_t slots = 0;              // partial slots (tile pieces)
-    double shared_us = 0, apart_us = 0;   // estimates: with these groups, without any
     int32_t step_pages = 0;         // pages of one step of the prefix kernel
     int64_t item_steps = 1;         // steps of the longest work item (choose_pieces)
     int32_t suffix_ctas = 0;        // SMs left to the suffix's decode beside the prefix kernel, 0: it runs behind it
@@ -66,8 +65,16 @@ void find_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t w
 pd_status check_prefix_groups(const pd_layout &layout, const int32_t *table, int64_t width, const int32_t *lengths,
                               const std::vector<PrefixGroup> &groups);
 
-// How the groups' work is cut (item_steps) and which SMs the suffix gets
-// (suffix_ctas), from the groups and the suffix's pages.
+// What follows from the layout and the type alone (group, item_words, step_pages).
+void set_shape(pd_prefix_plan &p);
+
+// Of the found groups, those that an estimate of the call's time says are worth it:
+// the ones that save the most page reads, as long as more of them make the call
+// shorter (all, some or none).  suffix_pages: the pages outside of all groups.
+void keep_paying_groups(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count);
+
+// How the groups' work is cut (tile_rows, item_steps) and which SMs the suffix gets
+// (suffix_ctas), from the groups and the pages outside of them.
 void choose_pieces(pd_prefix_plan &p, int64_t suffix_pages, int32_t sm_count);
 
 // Lay the groups' work out and build the device image; the suffix plan is set.

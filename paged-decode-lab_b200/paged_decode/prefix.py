@@ -127,8 +127,8 @@ class SharedPrefixPlan:
     ``layout``, ``table`` and ``lengths`` as for ``DecodePlan``.  ``prefixes``
     lists the groups as (sequence indices, pages): each sequence in at most one
     group, whose first ``pages`` pages are the same and whole in all of them;
-    None takes those of ``find_prefixes`` where the plan's estimate says that sharing is
-    faster (the decode kernel reads the copies of a short prefix from L2 in less time), []
+    None takes those of ``find_prefixes`` that make a call shorter by the plan's
+    estimate (the decode kernel reads the copies of a short prefix from L2 in less time), []
     shares nothing.  ``max_lengths`` makes a dynamic plan (``run_dynamic``).  ``run``
     returns the plan's own [batch, query_heads, head_dim] output in ``dtype``
     (the inputs' type; sums are FP32), which the next run overwrites.  Launch a
