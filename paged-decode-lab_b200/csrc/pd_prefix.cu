@@ -474,6 +474,7 @@ pd_status decode_impl(pd_prefix_plan *p, const void *q, const void *k, const voi
 pd_status create_impl(const pd_layout *layout, const int32_t *table, int64_t width, const int32_t *lengths,
                       const int32_t *max_lengths, int32_t group_count, const int32_t *indptr, const int32_t *members,
                       const int32_t *pages, pd_dtype dtype, int32_t device, pd_prefix_plan &p) {
+    if (group_count < -2) return fail(PD_ERR_VALUE, "group_count must be -2, -1 or a number of groups");
     // the decode plan's own checks of layout, table and lengths, before the groups look at them
     pd_plan *whole = nullptr;
     pd_status s = create_suffix_plan(layout, table, width, lengths, max_lengths, nullptr, dtype, -1, 0, &whole);

@@ -1,7 +1,10 @@
 """What the Python side hands to the prefix plan builder (no GPU)."""
+import ctypes
+
 import numpy as np
 import pytest
 
+from paged_decode import _native
 from paged_decode.layout import Layout
 from paged_decode.prefix import find_prefixes, inspect_prefix_plan
 
@@ -56,3 +59,16 @@ def test_types_by_name_or_as_torch_has_them():
     for bad in ("bfloat16", torch.bfloat16, None):
         with pytest.raises(TypeError, match="float16 or float32"):
             find_prefixes(LAYOUT, TABLE, LENGTHS, dtype=bad)
+
+
+def test_group_counts_below_the_two_that_mean_something():
+    lib = _native.load()
+    layout = _native.Layout(5, 8, 2, 64, 16, 40)
+    table, lengths = np.ascontiguousarray(TABLE, np.int32), np.ascontiguousarray(LENGTHS, np.int32)
+    for count, status in ((-1, _native.PD_OK), (-2, _native.PD_OK), (-3, _native.PD_ERR_VALUE),
+                          (-2 ** 31, _native.PD_ERR_VALUE)):
+        handle = ctypes.c_void_p()
+        got = lib.pd_prefix_plan_create(ctypes.byref(layout), table.ctypes.data, 5, lengths.ctypes.data, None, count,
+                                        None, None, None, 0, -1, ctypes.byref(handle))
+        assert got == status and bool(handle) == (status == _native.PD_OK)
+        lib.pd_prefix_plan_destroy(handle)
