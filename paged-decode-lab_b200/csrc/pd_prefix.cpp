@@ -147,7 +147,8 @@ std::vector<GroupShape> shapes_of(const std::vector<PrefixGroup> &groups) {
     for (const PrefixGroup &g : groups) ++counts[{int64_t(g.members.size()), int64_t(g.pages)}];
     std::vector<GroupShape> shapes;
     for (const auto &c : counts) shapes.push_back({c.first.first, c.first.second, c.second});
-    std::stable_sort(shapes.begin(), shapes.end(), [](const GroupShape &a, const GroupShape &b) { return a.saved() > b.saved(); });
+    std::stable_sort(shapes.begin(), shapes.end(),
+                     [](const GroupShape &a, const GroupShape &b) { return a.saved() > b.saved(); });
     return shapes;
 }
 

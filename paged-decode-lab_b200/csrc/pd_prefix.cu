@@ -14,6 +14,7 @@
 
 #include "paged_decode.h"
 #include "pd_device.cuh"
+#include "pd_launch.cuh"
 #include "pd_prefix.hpp"
 #include "pd_prefix_args.cuh"
 #include "pd_prefix_merge.cuh"
@@ -314,22 +315,6 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
         }
     }
     if (on) store_row<Elt, D>(sum, a, out_row, lane);
-}
-
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, unsigned threads, size_t smem,
-                             cudaStream_t stream, const Args &...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(grid));
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 using MmaKernel = void (*)(const CUtensorMap, const CUtensorMap, const PrefixArgs);

@@ -26,7 +26,8 @@
 // by more than 2^15 (then O is rescaled in tensor memory): a fresh reference is
 // 2^7 below the step's maximum, so weights stay within (0, 2^15] and FP16 keeps
 // its full precision down to 2^-21 of the largest.  The denominator sums the
-// FP32 weights.  Rows are either in use for the whole prefix or their results
+// rounded weights, as the warp-level decode kernel does, so that o / l stays an average
+// of the values (both in FP32).  Rows are either in use for the whole prefix or their results
 // are dropped (a live length inside the prefix, or other pages there: the merge kernel's slow path),
 // so no scores need masks; a last step of fewer pages takes fewer columns.
 //
@@ -490,7 +491,8 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                     store_sector(dst + (c / 8 + 1) * (S::M * 8), o + 8);
                 }
             }
-            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, LIVE && moved[t * S::M + first_row] ? kPieceMoved : l.x + l.y);
+            const bool usable = !LIVE || !moved[t * S::M + first_row];
+            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, usable ? l.x + l.y : kPieceMoved);
         }
         tc::fence_before_sync();
     }

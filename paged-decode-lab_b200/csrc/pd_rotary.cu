@@ -15,14 +15,13 @@
 // 32:32 FP32 heads of 64 21.6 us (135 MB, 6.2 TB/s); 64 tokens of 32:1 3.2 us
 // and 4 tokens into the cache 3.5 us, a launch and three trips to memory.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
-#include <mutex>
-#include <set>
 #include <string>
-#include <utility>
 
 #include "paged_decode.h"
 #include "pd_device.cuh"
+#include "pd_launch.cuh"
 #include "pd_plan.hpp"
 
 #define PD_API extern "C" __attribute__((visibility("default")))
@@ -374,13 +373,15 @@ struct StreamShape {
 // Streaming kernel: tokens whose rows lie one after another (16-byte aligned).
 // The bulk copies keep three stages per CTA in flight without registers (loads
 // into registers reached 2.8 TB/s), and three CTAs per SM of eight consumer warps
-// leave enough of them to hide the norm's exchanges (two CTAs 4.5 TB/s, four 5.0).  A persistent CTA takes every gridDim-th token through a ring of
-// stages: the producer warp brings a token's queries, keys, values and its
-// row of the rotation table by bulk copies, the consumer warps norm and rotate
-// the rows where they are, and the producer sends the whole token on by bulk
-// stores.  Places are looked up by the producer's lanes, 32 tokens at a time.
+// leave enough of them to hide the norm's exchanges (two CTAs 4.5 TB/s, four 5.0).
+// A persistent CTA takes every gridDim-th token through a ring of stages: the
+// producer warp brings a token's queries, keys, values and its row of the rotation
+// table by bulk copies, the consumer warps norm and rotate the rows where they are,
+// and the producer sends the whole token on by bulk stores.  Places are looked up
+// by the producer's lanes, 32 tokens at a time.
 template <typename Elt, int D, bool APPEND, bool INTERLEAVED>
-__global__ void __launch_bounds__(kStreamThreads, kStreamCtas) rotary_stream_kernel(const __grid_constant__ RotaryArgs a, const __grid_constant__ StreamShape sh) {
+__global__ void __launch_bounds__(kStreamThreads, kStreamCtas)
+    rotary_stream_kernel(const __grid_constant__ RotaryArgs a, const __grid_constant__ StreamShape sh) {
     using L = Lane<Elt, D, INTERLEAVED>;
     constexpr int H = L::H, W = L::W, LANES = L::LANES, PER_WARP = L::PER_WARP;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -525,34 +526,6 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamCtas) rotary_stream_ker
     }
 }
 
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), int64_t grid, int threads, size_t smem, cudaStream_t stream,
-                             const Args &...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(grid));
-    cfg.blockDim = dim3(unsigned(threads));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-// The streaming kernels whose dynamic shared memory was raised, per device.
-std::mutex g_stream_mutex;
-std::set<std::pair<int, const void *>> g_stream_done;
-
-cudaError_t allow_stream_smem(int device, const void *kernel) {
-    std::lock_guard<std::mutex> lock(g_stream_mutex);
-    if (g_stream_done.count({device, kernel})) return cudaSuccess;
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes[1] + 1024);
-    if (err == cudaSuccess) g_stream_done.insert({device, kernel});
-    return err;
-}
-
 // What a call's operands allow: whole 8-byte pieces, whole 16-byte aligned rows one after another.
 struct Alignment {
     bool pieces = true, rows = true;
@@ -581,8 +554,13 @@ cudaError_t launch_rotary(const RotaryArgs &a, Alignment align, int device, cuda
         sh.stages = std::min(kMaxStages, kRingBytes[ctas] / sh.stage_bytes);
         sh.smem = size_t(sh.stages) * sh.stage_bytes + kMaxStages * (8 + 8 + 8 + 4);
         const auto kernel = rotary_stream_kernel<Elt, D, APPEND, INTERLEAVED>;
-        err = allow_stream_smem(device, reinterpret_cast<const void *>(kernel));
-        if (err != cudaSuccess) return err;
+        static std::atomic<uint64_t> allowed{0};    // devices on which this kernel may use its shared memory
+        const uint64_t bit = unsigned(device) < 64 ? uint64_t(1) << device : 0;
+        if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes[1] + 1024);
+            if (err != cudaSuccess) return err;
+            allowed.fetch_or(bit, std::memory_order_relaxed);
+        }
         return launch_dependent(kernel, std::min<int64_t>(a.tokens, int64_t(ctas) * sms), kStreamThreads, sh.smem,
                                 stream, a, sh);
     }
