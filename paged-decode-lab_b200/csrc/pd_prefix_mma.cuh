@@ -37,10 +37,11 @@
 //
 // Bound by the tensor core and the exponentials alike: a 64-token step of both
 // streams counts 1280 cycles of MMAs (if scores of N 64 read shared memory at its
-// limit) and 1024 of ex2.  Measured on a B200, between lengths of 4096 and 32768 tokens
-// (256 sequences of 64:8 heads of 128, 128 CTAs): 0.87 to 0.92 us a step of both streams, 1.23
-// PFLOP/s; with few rows the loads bound it: 8 sequences of 32:8 heads behind 131072
-// tokens 94 us with the merge, 5.7 TB/s.
+// limit) and 1024 of ex2.  Measured on a B200, between lengths of 16384 and 65536
+// tokens (256 sequences of 64:8 heads of 128, 128 CTAs): 0.95 us a step of both streams, 1.13
+// PFLOP/s (0.87 and 1.23 with the unrounded weights' sum, two of which take one addition; up
+// to 12288 tokens the times are alike); with few rows the loads bound it: 8 sequences of 32:8 heads behind
+// 131072 tokens 91 us with the merge, 5.9 TB/s.
 //
 // Every wait is bounded; on a timeout the CTA records PD_DEVERR_TIMEOUT,
 // unwinds, waits for its own MMAs and copies and frees its tensor memory.
@@ -85,6 +86,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// x += the low FP16 of v, y += the high one, in FP32.
+__device__ __forceinline__ void add_halves(float &x, float &y, uint32_t v) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tadd.rn.f32.f16 %0, a, %0;\n\tadd.rn.f32.f16 %1, b, %1;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "r"(v));
 }
 
 // 32 bytes: a whole sector by one thread.
@@ -378,7 +386,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             return __all_sync(kFullMask, mbar_wait(smem_u32(bar), uint32_t(parity)));
         };
         float m = -INFINITY;                            // the row's reference
-        unsigned long long l2 = 0, l3 = 0;              // four partial denominators
+        float l[4] = {0.f, 0.f, 0.f, 0.f};              // partial denominators
         bool ok = true;
         for (int i = 0; i < n; ++i) {
             int32_t ids[NP];                            // the difference to the planned ones
@@ -436,31 +444,35 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                     }
                     tc::wait_st();
                 }
-                l2 = mul_f32x2(l2, pack_f32x2(f, f));
-                l3 = mul_f32x2(l3, pack_f32x2(f, f));
+#pragma unroll
+                for (int c = 0; c < 4; ++c) l[c] *= f;
                 m = next;
             }
             const float base = m == -INFINITY ? 0.f : m;
             const unsigned long long scale2 = pack_f32x2(a.scale_log2, a.scale_log2), base2 = pack_f32x2(-base, -base);
             // 32 weights of x or y into columns [16 c, 16 c + 16) of the block
-            const auto emit = [&](const uint32_t (&v)[32], int c, unsigned long long &sum) {
-                uint32_t p[16];
+            uint32_t px[16], py[16];
+            const auto emit = [&](const uint32_t (&v)[32], int c, uint32_t (&p)[16]) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float2 z = unpack_f32x2(fma_f32x2(
                         pack_f32x2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), scale2, base2));
                     p[e] = pack_half2(ex2_approx(z.x), ex2_approx(z.y));
-                    const float2 w = unpack_half2(p[e]);        // as the product sees them
-                    sum = add_f32x2(sum, pack_f32x2(w.x, w.y));
                 }
                 tc::st_32x32b_x16(block + 16 * c, p);
             };
-            emit(x, 0, l2);
-            emit(y, 1, l3);
+            emit(x, 0, px);
+            emit(y, 1, py);
             tc::wait_st();
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(p_full + 2 * t + (i & 1)));
+            // the denominator, of the weights as the product has them, while that runs
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                add_halves(l[0], l[1], px[e]);
+                add_halves(l[2], l[3], py[e]);
+            }
 #pragma unroll
             for (int p = 0; p < NP; ++p) other = other || ids[p] != 0;
         }
@@ -476,7 +488,6 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
             if (!ok && lane == 0) fail_wait();
         }
         tc::fence_after_sync();
-        const float2 l = unpack_f32x2(add_f32x2(l2, l3));
         const bool on = n > 0 && ok && member < it.members;
         if (n > 0) {
             // partials lie [D / 8][rows][8]: a row's reads take whole sectors, as do a thread's stores
@@ -492,7 +503,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 }
             }
             const bool usable = !LIVE || !moved[t * S::M + first_row];
-            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, usable ? l.x + l.y : kPieceMoved);
+            if (on) a.part_ml[int64_t(st.slot) * S::M + r] = make_float2(m, usable ? (l[0] + l[2]) + (l[1] + l[3]) : kPieceMoved);
         }
         tc::fence_before_sync();
     }
