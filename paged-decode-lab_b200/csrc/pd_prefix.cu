@@ -243,16 +243,13 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
     if (!a.rows && on && way == 0 && lane == 0 && __ldcg(a.lengths + b) > __ldg(a.seqs + 2 * b + 1).y)
         atomicOr(a.error, PD_DEVERR_LENGTH);
     // A dynamic launch's sequence that ends inside its prefix: pieces before its end count.
-    const int steps = (prefix_pages + a.step_pages - 1) / a.step_pages, count = pieces;
-    const auto start_of = [&](int p) {      // the first token of piece p, as the plan cuts them
-        return min(prefix_pages, p * steps / count * a.step_pages) * a.page_size;
-    };
+    const int count = pieces;
     int live = prefix_pages * a.page_size;
     if (LIVE && count > 0) {
         const int length = __ldcg(a.lengths + b);
         if (length < live) {
             live = length;
-            while (pieces > 0 && start_of(pieces) > live) --pieces;
+            while (pieces > 0 && piece_start(a, prefix_pages, count, pieces) > live) --pieces;
         }
     }
     bool moved = false;                     // a piece whose pages are others in the live table
@@ -281,22 +278,15 @@ __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __
             }
         }
 #pragma unroll
-        for (int j = 0; j < BATCH; ++j)
-            if (!LIVE || st[j].y != kPieceMoved) sum.add(st[j], u[j], v[j]);
-    }
-    if (LIVE && (moved || pieces < count)) {    // the other pieces, token by token
-        float o[8];
-        const int kv_head = head / a.group;
-        for (int p = way; p < pieces; p += ways)
-            if (__ldcg(ml + p * ml_step).y == kPieceMoved) {
-                const float2 st = walk<Elt, D>(a, out_row, kv_head, b, start_of(p), start_of(p + 1), kWalk, lane, o);
-                sum = joined(sum, st, o);
-            }
-        if (pieces < count) {               // the piece that the sequence ends in: all sets
-            const float2 st = walk<Elt, D>(a, out_row, kv_head, b, start_of(pieces) + way * kWalk, live, kWalk * ways,
-                                           lane, o);
-            sum = joined(sum, st, o);
+        for (int j = 0; j < BATCH; ++j) {
+            if (LIVE && st[j].y == kPieceMoved) st[j] = make_float2(-INFINITY, 0.f);
+            sum.add(st[j], u[j], v[j]);
         }
+    }
+    if (LIVE && (moved || pieces < count)) {
+        RowSum all = sum;
+        add_others<Elt, D>(all, a, out_row, head / a.group, b, ml, prefix_pages, count, pieces, live, way, ways, lane);
+        sum = all;
     }
     if (ways > 1) {
         float *mine = sums[threadIdx.x];

@@ -143,4 +143,31 @@ __device__ __forceinline__ void store_row(RowSum &sum, const PrefixArgs &a, int6
     store8(static_cast<Elt *>(a.out) + row * D + lane * 8, sum.o);
 }
 
+// The first token of piece p of `count`, as the plan cuts them.
+__device__ __forceinline__ int piece_start(const PrefixArgs &a, int prefix_pages, int count, int p) {
+    const int steps = (prefix_pages + a.step_pages - 1) / a.step_pages;
+    return min(prefix_pages, p * steps / count * a.step_pages) * a.page_size;
+}
+
+// A dynamic launch's pieces that the group's matrix does not describe, token by token: of the first
+// `whole` those whose pages are others now (each by the set that has it), and the one that the
+// sequence ends in, at token `live` (by all sets).
+template <typename Elt, int D>
+__device__ __noinline__ void add_others(RowSum &sum, const PrefixArgs &a, int64_t row, int kv_head, int b,
+                                        const float2 *ml, int prefix_pages, int count, int whole, int live, int way,
+                                        int ways, int lane) {
+    float o[8];
+    for (int p = way; p < whole; p += ways)
+        if (__ldcg(ml + int64_t(p) * a.tile_rows).y == kPieceMoved) {
+            const float2 st = walk<Elt, D>(a, row, kv_head, b, piece_start(a, prefix_pages, count, p),
+                                           piece_start(a, prefix_pages, count, p + 1), kWalk, lane, o);
+            sum = joined(sum, st, o);
+        }
+    if (whole < count) {
+        const float2 st = walk<Elt, D>(a, row, kv_head, b, piece_start(a, prefix_pages, count, whole) + way * kWalk, live,
+                                       kWalk * ways, lane, o);
+        sum = joined(sum, st, o);
+    }
+}
+
 }  // namespace pd

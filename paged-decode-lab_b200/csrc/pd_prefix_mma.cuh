@@ -95,6 +95,13 @@ __device__ __forceinline__ void add_halves(float &x, float &y, uint32_t v) {
         : "r"(v));
 }
 
+// A read-only load that stays where it is written: its result is used much later.
+__device__ __forceinline__ int32_t load_here(const int32_t *p) {
+    int32_t r;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(p));
+    return r;
+}
+
 // 32 bytes: a whole sector by one thread.
 __device__ __forceinline__ void store_sector(void *p, const uint32_t *r) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
@@ -373,13 +380,15 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         const int row = st.tile * S::M + r, member = row / a.group;
         const int first_row = max(0, member * a.group - st.tile * S::M);
         const int32_t *live_ids = nullptr, *planned_ids = a.pages + it.page0 + st.first;
-        unsigned mine = 0;                              // this thread's pages of a step
+        const int mate = r - first_row, mates = min(S::M, (member + 1) * a.group - st.tile * S::M) - first_row;
         bool other = false;
-        if (LIVE && member < it.members && n > 0) {
-            const int mates = min(S::M, (member + 1) * a.group - st.tile * S::M) - first_row;
+        if (LIVE && member < it.members && mate < NP)
             live_ids = a.table + __ldg(a.members + it.member0 + member) * a.width + st.first;
-            for (int p = r - first_row; p < NP; p += mates) mine |= 1u << p;
-        }
+        if (LIVE && live_ids)           // a member with fewer rows than a step has pages: the others at once
+            for (int p = mate + mates; p < NP; p += mates)
+#pragma unroll 4
+                for (int at = p; at < st.end - st.first; at += NP)
+                    other = other | (__ldg(live_ids + at) != __ldg(planned_ids + at));
         const uint32_t lanes = uint32_t(32 * quad) << 16;
         const uint32_t ts = tmem + lanes + S::S_COL + 2 * t * S::NS, to = tmem + lanes + S::O_COL + t * D;
         const auto warp_wait = [&](uint64_t *bar, int parity) {
@@ -389,12 +398,10 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
         float l[4] = {0.f, 0.f, 0.f, 0.f};              // partial denominators
         bool ok = true;
         for (int i = 0; i < n; ++i) {
-            int32_t ids[NP];                            // the difference to the planned ones
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                const int at = i * NP + p;
-                const bool on = LIVE && (mine >> p & 1) && at < st.end - st.first;
-                ids[p] = on ? __ldg(live_ids + at) ^ __ldg(planned_ids + at) : 0;
+            int32_t id = 0, planned = 0;                // of page `mate` of the step; compared at its end
+            if (LIVE && live_ids) {
+                const int end = min((i + 1) * NP, st.end - st.first), at = i * NP + mate;
+                if (at < end) id = load_here(live_ids + at), planned = load_here(planned_ids + at);
             }
             if (!warp_wait(s_full + 2 * t + (i & 1), i >> 1 & 1)) {
                 ok = false;
@@ -473,8 +480,7 @@ __global__ void __launch_bounds__(PrefixShape<D, T>::THREADS, 1)
                 add_halves(l[0], l[1], px[e]);
                 add_halves(l[2], l[3], py[e]);
             }
-#pragma unroll
-            for (int p = 0; p < NP; ++p) other = other || ids[p] != 0;
+            if (LIVE) other = other || id != planned;
         }
         if (LIVE) {
             if (other) moved[t * S::M + first_row] = 1;

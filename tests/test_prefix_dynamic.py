@@ -188,3 +188,25 @@ def test_a_length_inside_a_long_prefix_costs_a_piece_of_it(dtype):
             times[name] = min(times[name], begin.elapsed_time(end))
     close(out[2:3], *exact(q[2:3], k, v, table[2:3], short[2:3]))
     assert times["short"] < 25 * times["planned"], times
+
+
+@pytest.mark.parametrize("heads,kv,sharers", [(10, 2, 60), (4, 4, 140), (2, 1, 67), (21, 7, 45)])
+@pytest.mark.parametrize("page", [16, 32])
+def test_every_page_of_every_row_tile_is_looked_at(heads, kv, sharers, page):
+    """Members with few rows, and ones whose rows lie in two tiles: one page at a time moves for one of them."""
+    shared, D = 11, 64
+    layout, table, lengths, spare, q, k, v = serving_batch(sharers, shared, 0, heads, kv, D, page, F16)
+    plan = SharedPrefixPlan(layout, table, lengths, prefixes=[(range(sharers), shared)],
+                            max_lengths=np.full(layout.batch, table.shape[1] * page))
+    before = plan.run_dynamic(q, k, v, cuda(table), cuda(lengths)).clone()
+    group = heads // kv
+    edges = {m for m in range(sharers) if m * group // 128 != ((m + 1) * group - 1) // 128}
+    for m in sorted(edges | {0, sharers - 1}):
+        for p in range(shared):
+            live = table.copy()
+            live[m, p] = spare[p]
+            out = plan.run_dynamic(q, k, v, cuda(live), cuda(lengths))
+            close(out[m:m + 1], *exact(q[m:m + 1], k, v, live[m:m + 1], lengths[m:m + 1]))
+            same = np.arange(sharers) != m
+            assert torch.equal(out[same], before[same]) and not torch.equal(out[m], before[m])
+    assert plan.read_errors() == 0
