@@ -214,9 +214,9 @@ __global__ void __launch_bounds__(kSimtThreads) prefix_simt_kernel(const __grid_
 // ways-th piece (several where rows are few and pieces many); the sets' parts are
 // merged in order.  What a row needs to know is looked up before the
 // kernels in front are waited for; pieces are loaded four at a time.  Bound by
-// latency: 18 us for 16384 rows of head_dim 128 when profiled alone on cold caches.
+// latency: 17 us for 16384 rows of head_dim 128 when profiled alone on cold caches.
+// LIVE: a dynamic launch; pieces that its lengths or table do not bear out are left to add_others.
 constexpr int kMergeThreads = 256;
-// LIVE: a dynamic launch.
 template <typename Elt, int D, bool LIVE>
 __global__ void __launch_bounds__(kMergeThreads, 3) prefix_merge_kernel(const __grid_constant__ PrefixArgs a, int ways) {
     constexpr int LANES = D / 8, BATCH = 4;
